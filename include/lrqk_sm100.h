@@ -365,6 +365,31 @@ int lrqk_rope_qkv(const void *qkv, const void *cos, const void *sin, int32_t cos
                   lrqk_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Rotary positions of q and k, forward and adjoint, from positions and frequencies (no cos/sin tables).  The
+ * reference leaves prompts to apply_rotary_pos_emb of the transformers modules (lrqk_attention.py:2275); this entry
+ * serves prompts, single tokens, drafted trees and re-positioned keys, with angles right for positions of millions.
+ *   pair (a, b), t = position * inv_freq[i]:  a' = factor (a cos t - b sin t),  b' = factor (b cos t + a sin t);
+ *   (a, b) = (x[i], x[i + rotary_dim/2]), or (x[2i], x[2i+1]) when interleaved; elements from rotary_dim on are copied;
+ *   adjoint: t -> -t (the gradient with respect to x).  fp32 arithmetic, one rounding to `dtype`.
+ *   q [batch, q_heads, length, head_dim] and k [batch, k_heads, length, head_dim] with the strides given (elements; the
+ *   last dimension is dense); q_out, k_out dense in that shape and not overlapping the sources.  k_heads = 0: q alone.
+ *   positions: [batch, length], position_stride elements between sequences (0: one row for all), int64 or int32, of
+ *   either sign.  inv_freq: device double [rotary_dim / 2], radians per position.
+ * ---------------------------------------------------------------------------------- */
+typedef struct lrqk_rotary_args {
+  int32_t dtype, batch, length, q_heads, k_heads, head_dim, rotary_dim;
+  int32_t interleaved, adjoint, positions_are_64bit;
+  const void *q, *k;
+  int64_t q_stride[3], k_stride[3]; /* batch, head, token */
+  void *q_out, *k_out;
+  const void *positions;
+  int64_t position_stride;
+  const double *inv_freq;
+  float factor;
+} lrqk_rotary_args;
+int lrqk_rotary(const lrqk_rotary_args *a, lrqk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * Element-wise glue of a decoder layer around the attention call, for the decode step (one token per
  * sequence), where every eager framework op is one launch of pure latency.  The reference leaves these to
  * the transformers modules (LlamaRMSNorm / Qwen2RMSNorm / MistralRMSNorm forward, the residual adds of the

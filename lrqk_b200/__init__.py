@@ -36,7 +36,10 @@ from .extras import (  # noqa: F401,E402
     tps_estimate,
 )
 
+from .rotary import apply_rotary, rotary_frequencies  # noqa: F401,E402
+
 __all__ = [
+    "apply_rotary", "rotary_frequencies",
     "FullOffloadCache", "HitRateCounter", "LightAttentionIndicesOffloadPrefill", "WrapForwardTimer", "run_task",
     "tps_estimate",
     "load_lrqk_model", "load_model", "load_model_hack", "load_tokenizer", "lrqk_attention_forward", "lrqk_decoder_layer_forward", "patch_model",

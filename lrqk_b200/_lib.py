@@ -66,6 +66,17 @@ class PeerGroup(C.Structure):
     ]
 
 
+class RotaryArgs(C.Structure):
+    """struct lrqk_rotary_args."""
+    _fields_ = [
+        ("dtype", C.c_int32), ("batch", C.c_int32), ("length", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32),
+        ("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("adjoint", C.c_int32),
+        ("positions_are_64bit", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p), ("q_stride", C.c_int64 * 3),
+        ("k_stride", C.c_int64 * 3), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("positions", C.c_void_p),
+        ("position_stride", C.c_int64), ("inv_freq", C.c_void_p), ("factor", C.c_float),
+    ]
+
+
 _SIGNATURES = {
     # name: (restype, argtypes)
     "lrqk_version": (C.c_char_p, []),
@@ -121,6 +132,7 @@ _SIGNATURES = {
     "lrqk_rope_qkv": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                 C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
                                 C.c_void_p]),
+    "lrqk_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
     "lrqk_add_rmsnorm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_float, C.c_int32, C.c_int32, C.c_int32,
                                    C.c_void_p, C.c_void_p, C.c_void_p]),
     "lrqk_swiglu": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
