@@ -390,6 +390,40 @@ typedef struct lrqk_rotary_args {
 int lrqk_rotary(const lrqk_rotary_args *a, lrqk_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Attention of a tree of drafted tokens over a cache (no counterpart in the reference, whose decode step takes one
+ * token, lrqk_attention.py:1506-1613): stands beside lrqk_flash_decode for the verification of several drafted tokens in
+ * one call.  Node i of sequence b attends to rows [0, cache_lens[b]) of the cache and to the drafted nodes j with
+ * mask[b][i][j] != 0.  Changes no cache.
+ *   q [batch, q_heads, nodes, d], cache_k / cache_v [batch, cache_heads, capacity, d], tree_k / tree_v [batch,
+ *   tree_heads, nodes, d]: strides in elements (batch, head, row; 0 allowed), last dimension dense, every row on 16
+ *   bytes.  tree_heads divides cache_heads divides q_heads: the resident rows of a decoding layer have cache_heads =
+ *   q_heads, an ordinary cache cache_heads = tree_heads = the KV heads.
+ *   cache_lens : device int32 [batch], read when the kernel runs and cut to [0, capacity]; NULL: capacity.  Rows behind
+ *                a length are not used and may hold anything, as may nodes that no node sees.
+ *   mask       : bytes [nodes][nodes] per sequence, mask_stride bytes apart (0: one for all); NULL: node i sees 0..i.
+ *   out        : dense [batch, q_heads, nodes, d]; lse: optional dense fp32 [batch, q_heads, nodes], natural
+ *                logarithm of the sum of exponentials.  A row that sees nothing gives zeros and -infinity.
+ *   status     : optional device int32, zero before the first call: takes LRQK_ETIMEOUT if a bounded wait ran out; as
+ *                long as it is set, calls hand out NaN rows.
+ *   head_dim 64 or 128, up to 256 nodes.  The workspace needs no initialisation.
+ * ---------------------------------------------------------------------------------- */
+typedef struct lrqk_tree_args {
+  int32_t dtype, batch, nodes, q_heads, cache_heads, tree_heads, head_dim;
+  float scale;              /* > 0 */
+  int64_t capacity;
+  const void *q, *cache_k, *cache_v, *tree_k, *tree_v;
+  int64_t q_stride[3], cache_k_stride[3], cache_v_stride[3], tree_k_stride[3], tree_v_stride[3];
+  const int32_t *cache_lens;
+  const uint8_t *mask;
+  int64_t mask_stride;
+  void *out;
+  float *lse;
+  int32_t *status;
+} lrqk_tree_args;
+size_t lrqk_tree_attention_workspace_bytes(const lrqk_tree_args *a);
+int lrqk_tree_attention(const lrqk_tree_args *a, void *workspace, lrqk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * Element-wise glue of a decoder layer around the attention call, for the decode step (one token per
  * sequence), where every eager framework op is one launch of pure latency.  The reference leaves these to
  * the transformers modules (LlamaRMSNorm / Qwen2RMSNorm / MistralRMSNorm forward, the residual adds of the

@@ -77,6 +77,19 @@ class RotaryArgs(C.Structure):
     ]
 
 
+class TreeArgs(C.Structure):
+    """struct lrqk_tree_args."""
+    _fields_ = [
+        ("dtype", C.c_int32), ("batch", C.c_int32), ("nodes", C.c_int32), ("q_heads", C.c_int32), ("cache_heads", C.c_int32),
+        ("tree_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float), ("capacity", C.c_int64),
+        ("q", C.c_void_p), ("cache_k", C.c_void_p), ("cache_v", C.c_void_p), ("tree_k", C.c_void_p), ("tree_v", C.c_void_p),
+        ("q_stride", C.c_int64 * 3), ("cache_k_stride", C.c_int64 * 3), ("cache_v_stride", C.c_int64 * 3),
+        ("tree_k_stride", C.c_int64 * 3), ("tree_v_stride", C.c_int64 * 3),
+        ("cache_lens", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
+
+
 _SIGNATURES = {
     # name: (restype, argtypes)
     "lrqk_version": (C.c_char_p, []),
@@ -133,6 +146,8 @@ _SIGNATURES = {
                                 C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
                                 C.c_void_p]),
     "lrqk_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
+    "lrqk_tree_attention_workspace_bytes": (C.c_size_t, [C.POINTER(TreeArgs)]),
+    "lrqk_tree_attention": (C.c_int, [C.POINTER(TreeArgs), C.c_void_p, C.c_void_p]),
     "lrqk_add_rmsnorm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_float, C.c_int32, C.c_int32, C.c_int32,
                                    C.c_void_p, C.c_void_p, C.c_void_p]),
     "lrqk_swiglu": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),

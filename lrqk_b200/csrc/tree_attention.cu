@@ -1,0 +1,327 @@
+// Attention of a tree of drafted tokens over a cache:  out_i = sum_j softmax_j(scale q_i . k_j) v_j  with j over the
+// filled rows of the cache and the drafted nodes that node i sees.
+//
+// This file: the entry points, the fp32 kernel and the combine kernel.  (bf16 runs on the tensor cores,
+// tree_attention_tc.cu.)  One pass over the keys with a running maximum and sum; scores, weights and sums in fp32.
+//
+// The fp32 kernel keeps to fp32 multiply-adds (tf32 would cost three digits).  A CTA holds 64 query rows and walks 64-key
+// tiles: scores from 4 x 4 register tiles, weights through shared memory, 4 rows x head_dim/16 columns of the result in
+// registers.  Bound: fp32 FMA from about 16 rows a cache head on, HBM below.
+#include "tree_plan.cuh"
+
+namespace lrqk {
+namespace tree {
+namespace {
+
+constexpr int kRows = 64, kKeys = 64, kThreads = 256;
+
+template <int D> struct SimtShared {
+  float q[kRows][D], k[kKeys][D + 4], v[kKeys][D], w[kRows][kKeys + 1];
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_constant__ Params p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  SimtShared<D> &sm = *reinterpret_cast<SimtShared<D> *>(smem_raw);
+  constexpr int VE = Elt<T>::kPerVec, DC = D / 64;      // columns of a thread: DC runs of four
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int group = blockIdx.x / p.row_blocks, block = blockIdx.x % p.row_blocks;
+  int64_t before, total;
+  count_tiles(p, 0, before, total);
+  const int64_t x0 = group_start(p, total, group), x1 = group_start(p, total, group + 1);
+  int seq = 0;
+  int64_t base = 0;
+  if (x0 < x1) find_sequence(p, x0, seq, base);
+  const int row0 = block * kRows, n_rows = min(kRows, p.rows - row0), per_head = p.q_heads / p.cache_heads;
+  const bool works = ty * 4 < n_rows;                   // rows of this thread exist
+
+  for (Walk w(p, x0, x1, seq, base); w.valid(); w.next(p)) {
+    __syncthreads();
+    for (int i = tid; i < kRows * (D / VE); i += kThreads) {
+      const int r = i / (D / VE), c = i % (D / VE) * VE;
+      float f[VE] = {};
+      if (r < n_rows) {
+        const int g = (row0 + r) / p.nodes, t = (row0 + r) % p.nodes;
+        Elt<T>::unpack(ld16(static_cast<const T *>(p.q) + w.b * p.q_stride[0] + (int64_t)(w.head * per_head + g) * p.q_stride[1] + t * p.q_stride[2] + c), f);
+      }
+#pragma unroll
+      for (int j = 0; j < VE; ++j) sm.q[r][c + j] = f[j];
+    }
+    float top[4], sum[4], acc[4][4 * DC];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      top[i] = -INFINITY;
+      sum[i] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 4 * DC; ++c) acc[i][c] = 0.0f;
+    }
+    const int tree_head = w.head / (p.cache_heads / p.tree_heads);
+    for (int tile = w.t0; tile < w.t1; ++tile) {
+      const bool drafted = tile >= w.ctiles;
+      const int first = (drafted ? tile - w.ctiles : tile) * kKeys;
+      const int n_keys = min(kKeys, (drafted ? p.nodes : w.len) - first);
+      const T *gk = drafted ? static_cast<const T *>(p.tree_k) + w.b * p.tk_stride[0] + tree_head * p.tk_stride[1]
+                            : static_cast<const T *>(p.cache_k) + w.b * p.ck_stride[0] + w.head * p.ck_stride[1];
+      const T *gv = drafted ? static_cast<const T *>(p.tree_v) + w.b * p.tv_stride[0] + tree_head * p.tv_stride[1]
+                            : static_cast<const T *>(p.cache_v) + w.b * p.cv_stride[0] + w.head * p.cv_stride[1];
+      const int64_t sk = drafted ? p.tk_stride[2] : p.ck_stride[2], sv = drafted ? p.tv_stride[2] : p.cv_stride[2];
+      __syncthreads();
+      for (int i = tid; i < kKeys * (D / VE); i += kThreads) {
+        const int r = i / (D / VE), c = i % (D / VE) * VE;
+        float fk[VE] = {}, fv[VE] = {};
+        if (r < n_keys) {                               // rows behind the filled ones are never read: they may hold anything
+          Elt<T>::unpack(ld16(gk + (int64_t)(first + r) * sk + c), fk);
+          Elt<T>::unpack(ld16(gv + (int64_t)(first + r) * sv + c), fv);
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j) { sm.k[r][c + j] = fk[j]; sm.v[r][c + j] = fv[j]; }
+      }
+      __syncthreads();
+      if (works) {                                      // whole half-warps: a row's 16 threads stay together
+        float s[4][4] = {};
+#pragma unroll 4
+        for (int c = 0; c < D; c += 4) {
+          float4 a[4], b[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4 *>(&sm.q[ty * 4 + i][c]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(&sm.k[tx + 16 * j][c]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+        }
+        const unsigned half = (tid & 16) ? 0xFFFF0000u : 0x0000FFFFu;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = row0 + ty * 4 + i, node = r % p.nodes;
+          float m = top[i];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int key = tx + 16 * j;
+            const bool seen = key < n_keys && r < p.rows && (!drafted || sees(p, w.b, node, first + key));
+            s[i][j] = seen ? s[i][j] * p.scale_log2 : -INFINITY;
+            m = fmaxf(m, s[i][j]);
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(half, m, o));
+          const float at = m == -INFINITY ? 0.0f : m, fade = exp2f(top[i] - at);   // a row that has seen nothing yet fades nothing
+          top[i] = m;
+          float add = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float e = exp2f(s[i][j] - at);
+            sm.w[ty * 4 + i][tx + 16 * j] = e;
+            add += e;
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) add += __shfl_xor_sync(half, add, o);
+          sum[i] = sum[i] * fade + add;
+#pragma unroll
+          for (int c = 0; c < 4 * DC; ++c) acc[i][c] *= fade;
+        }
+        __syncwarp(half);
+        for (int key = 0; key < n_keys; ++key) {
+          float4 v[DC];
+#pragma unroll
+          for (int c = 0; c < DC; ++c) v[c] = *reinterpret_cast<const float4 *>(&sm.v[key][tx * 4 + 64 * c]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = sm.w[ty * 4 + i][key];
+            if (drafted && e == 0.0f) continue;         // a node that the row does not see adds nothing, whatever it holds
+#pragma unroll
+            for (int c = 0; c < DC; ++c) {
+              acc[i][4 * c] = fmaf(e, v[c].x, acc[i][4 * c]);
+              acc[i][4 * c + 1] = fmaf(e, v[c].y, acc[i][4 * c + 1]);
+              acc[i][4 * c + 2] = fmaf(e, v[c].z, acc[i][4 * c + 2]);
+              acc[i][4 * c + 3] = fmaf(e, v[c].w, acc[i][4 * c + 3]);
+            }
+          }
+        }
+      }
+    }
+    if (!works) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = row0 + ty * 4 + i;
+      if (r >= p.rows) continue;
+      if (w.whole()) {
+        const int g = r / p.nodes, t = r % p.nodes;
+        const int64_t at = ((int64_t)w.b * p.q_heads + w.head * per_head + g) * p.nodes + t;
+        const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
+        T *dst = static_cast<T *>(p.out) + at * D;
+#pragma unroll
+        for (int c = 0; c < 4 * DC; ++c) dst[tx * 4 + 64 * (c / 4) + c % 4] = Elt<T>::from_float(acc[i][c] * inv);
+        if (p.lse && tx == 0) p.lse[at] = sum[i] == 0.0f ? -INFINITY : (top[i] + log2f(sum[i])) * 0.6931471805599453f;
+      } else {
+        const int64_t at = w.slot(p, group, block) * p.rows_per_block + (r - row0);
+#pragma unroll
+        for (int c = 0; c < DC; ++c)
+          *reinterpret_cast<float4 *>(p.part + at * D + tx * 4 + 64 * c) = make_float4(acc[i][4 * c], acc[i][4 * c + 1], acc[i][4 * c + 2], acc[i][4 * c + 3]);
+        if (tx == 0) p.part_ml[at] = make_float2(top[i], sum[i]);
+      }
+    }
+  }
+}
+
+// One warp per query row of a unit that was cut: the row's partials, folded in the order of the runs.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Params p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int E = D / 32;                             // columns of a lane
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= (int64_t)p.batch * p.q_heads * p.nodes) return;
+  const int t = (int)(row % p.nodes), h = (int)(row / p.nodes % p.q_heads), b = (int)(row / p.nodes / p.q_heads);
+  T *dst = static_cast<T *>(p.out) + row * D + lane * E;
+  if (p.status && *reinterpret_cast<volatile int32_t *>(p.status) != 0) {   // a wait ran out: no row can be trusted
+    for (int c = 0; c < E; ++c) dst[c] = Elt<T>::from_float(NAN);
+    if (p.lse && lane == 0) p.lse[row] = NAN;
+    return;
+  }
+  const int per_head = p.q_heads / p.cache_heads, head = h / per_head;
+  int64_t before, total;
+  count_tiles(p, b, before, total);
+  const int per = cache_tiles(p, cache_len(p, b)) + p.tree_tiles;
+  const int64_t u0 = before + (int64_t)head * per;
+  const int g0 = group_of(p, total, u0), g1 = group_of(p, total, u0 + per - 1);
+  if (g0 == g1) return;                                 // one run holds the unit: it is written already
+  const int r = (h - head * per_head) * p.nodes + t, block = r / p.rows_per_block, at = r % p.rows_per_block;
+  float top = -INFINITY, sum = 0.0f, acc[E] = {};
+  for (int first = g0; first <= g1; first += 32) {
+    // a lane holds one run's maximum and sum; runs without tiles (fewer tiles than runs) hold nothing
+    const int g = first + lane;
+    int64_t slot = 0;
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (g <= g1) {
+      const int64_t s0 = group_start(p, total, g), s1 = group_start(p, total, g + 1);
+      if (s0 < s1) {
+        slot = (((int64_t)g * 2 + (s0 >= u0 ? 0 : 1)) * p.row_blocks + block) * p.rows_per_block + at;
+        ml = p.part_ml[slot];
+      }
+    }
+    float m = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    m = fmaxf(m, top);
+    const float ref = m == -INFINITY ? 0.0f : m, fade = exp2f(top - ref);
+    const float weight = exp2f(ml.x - ref);
+    top = m;
+    sum *= fade;
+#pragma unroll
+    for (int c = 0; c < E; ++c) acc[c] *= fade;
+    const int n = min(32, g1 - first + 1);
+    for (int i = 0; i < n; ++i) {
+      const float wi = __shfl_sync(0xFFFFFFFFu, weight, i), si = __shfl_sync(0xFFFFFFFFu, ml.y, i);
+      const int64_t at_i = __shfl_sync(0xFFFFFFFFu, slot, i);
+      if (si == 0.0f) continue;                         // nothing seen there (or no tiles)
+      sum = fmaf(wi, si, sum);
+      const float *src = p.part + at_i * D + lane * E;
+#pragma unroll
+      for (int c = 0; c < E; ++c) acc[c] = fmaf(wi, src[c], acc[c]);
+    }
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int c = 0; c < E; ++c) dst[c] = Elt<T>::from_float(acc[c] * inv);
+  if (p.lse && lane == 0) p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+}
+
+template <typename T, int D> int launch_simt(const Params &p, cudaStream_t stream) {
+  static SmemOptIn opt_in;
+  auto kern = tree_simt_kernel<T, D>;
+  LRQK_CUDA_TRY(opt_in.ensure(kern, sizeof(SimtShared<D>)));
+  LRQK_CUDA_TRY(launch_dependent(kern, dim3((unsigned)(p.groups * p.row_blocks)), dim3(kThreads), sizeof(SimtShared<D>), stream, 0, p));
+  return LRQK_OK;
+}
+
+template <typename T, int D> int launch_combine(const Params &p, cudaStream_t stream) {
+  const int64_t rows = (int64_t)p.batch * p.q_heads * p.nodes;
+  LRQK_CUDA_TRY(launch_dependent(tree_combine_kernel<T, D>, dim3((unsigned)ceil_div64(rows, 8)), dim3(256), 0, stream, 0, p));
+  return LRQK_OK;
+}
+
+// The split of these arguments (no device work).
+int plan(const lrqk_tree_args *a, Params &p) {
+  if (!a) return LRQK_EINVAL;
+  if (a->dtype != LRQK_F32 && a->dtype != LRQK_BF16) return LRQK_EUNSUPPORTED;
+  if (a->batch <= 0 || a->nodes <= 0 || a->q_heads <= 0 || a->cache_heads <= 0 || a->tree_heads <= 0 || a->capacity < 0) return LRQK_EINVAL;
+  if (a->q_heads % a->cache_heads != 0 || a->cache_heads % a->tree_heads != 0) return LRQK_EINVAL;
+  if (a->head_dim != 64 && a->head_dim != 128) return LRQK_EUNSUPPORTED;
+  if (a->nodes > 256 || a->capacity >= (1ll << 31) - 256) return LRQK_EUNSUPPORTED;
+  if ((int64_t)a->batch * a->q_heads * a->nodes >= (1ll << 31)) return LRQK_EUNSUPPORTED;
+  p.batch = a->batch; p.nodes = a->nodes; p.q_heads = a->q_heads; p.cache_heads = a->cache_heads; p.tree_heads = a->tree_heads;
+  p.head_dim = a->head_dim; p.capacity = (int32_t)a->capacity;
+  p.rows = a->q_heads / a->cache_heads * a->nodes;
+  p.rows_per_block = kRows;
+  p.tile_keys = kKeys;
+  p.row_blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
+  // two CTAs an SM; the row blocks of a unit walk the same keys at the same time, so those are read from HBM once
+  p.groups = 2 * kNumSMs / p.row_blocks;
+  if (p.groups < 1) return LRQK_EUNSUPPORTED;
+  p.tree_tiles = (p.nodes + p.tile_keys - 1) / p.tile_keys;
+  return LRQK_OK;
+}
+
+size_t workspace_bytes(const Params &p) {
+  const size_t rows = (size_t)p.groups * 2 * p.row_blocks * p.rows_per_block;
+  return rows * p.head_dim * sizeof(float) + rows * sizeof(float2);
+}
+
+}  // namespace
+}  // namespace tree
+}  // namespace lrqk
+
+extern "C" {
+
+size_t lrqk_tree_attention_workspace_bytes(const lrqk_tree_args *a) {
+  lrqk::tree::Params p = {};
+  return lrqk::tree::plan(a, p) == LRQK_OK ? lrqk::tree::workspace_bytes(p) : 0;
+}
+
+int lrqk_tree_attention(const lrqk_tree_args *a, void *workspace, lrqk_stream_t stream) {
+  using namespace lrqk;
+  int rc = check_device();
+  if (rc != LRQK_OK) return rc;
+  tree::Params p = {};
+  rc = tree::plan(a, p);
+  if (rc != LRQK_OK) return rc;
+  if (!a->q || !a->tree_k || !a->tree_v || !a->out || !workspace) return LRQK_EINVAL;
+  if (a->capacity > 0 && (!a->cache_k || !a->cache_v)) return LRQK_EINVAL;
+  if (!(a->scale > 0.0f) || a->scale > 3.0e38f) return LRQK_EINVAL;
+  // 16-byte rows: what the kernels' loads need
+  uintptr_t low = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->tree_k) | reinterpret_cast<uintptr_t>(a->tree_v) |
+                  reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(workspace);
+  if (a->capacity > 0) low |= reinterpret_cast<uintptr_t>(a->cache_k) | reinterpret_cast<uintptr_t>(a->cache_v);
+  for (int i = 0; i < 3; ++i) {
+    p.q_stride[i] = a->q_stride[i];
+    p.ck_stride[i] = a->cache_k_stride[i];
+    p.cv_stride[i] = a->cache_v_stride[i];
+    p.tk_stride[i] = a->tree_k_stride[i];
+    p.tv_stride[i] = a->tree_v_stride[i];
+    const int64_t all = a->q_stride[i] | a->tree_k_stride[i] | a->tree_v_stride[i] |
+                        (a->capacity > 0 ? a->cache_k_stride[i] | a->cache_v_stride[i] : 0);
+    low |= (uintptr_t)(all * (int64_t)elt_size(a->dtype));
+    if (a->q_stride[i] < 0 || a->tree_k_stride[i] < 0 || a->tree_v_stride[i] < 0 || a->cache_k_stride[i] < 0 || a->cache_v_stride[i] < 0)
+      return LRQK_EINVAL;
+  }
+  if (low & 15) return LRQK_EUNSUPPORTED;
+  p.q = a->q; p.cache_k = a->cache_k; p.cache_v = a->cache_v; p.tree_k = a->tree_k; p.tree_v = a->tree_v;
+  p.lens = a->cache_lens; p.mask = a->mask; p.mask_stride = a->mask_stride;
+  p.out = a->out; p.lse = a->lse; p.status = a->status;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.part = static_cast<float *>(workspace);
+  p.part_ml = reinterpret_cast<float2 *>(p.part + (size_t)p.groups * 2 * p.row_blocks * p.rows_per_block * p.head_dim);
+  const cudaStream_t s = as_stream(stream);
+  LRQK_DISPATCH_DTYPE(a->dtype, T, {
+    rc = a->head_dim == 64 ? tree::launch_simt<T, 64>(p, s) : tree::launch_simt<T, 128>(p, s);
+    if (rc != LRQK_OK) return rc;
+    return a->head_dim == 64 ? tree::launch_combine<T, 64>(p, s) : tree::launch_combine<T, 128>(p, s);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,135 @@
+// Work split of the tree attention, shared by its kernels (tree_attention.cu, tree_attention_tc.cu).
+//
+// A unit is one (sequence, cache head) and one block of its query rows (rows = the G query heads that read the cache
+// head, times the nodes).  Its keys come in tiles: first the filled rows of the cache, then the drafted nodes.  All units'
+// tiles, laid end to end, are cut into `groups` equal runs, one per CTA, whatever the sequences' lengths are; those are read
+// on the device, so a captured call follows them.  A unit that falls into several runs leaves one partial result per
+// run (fp32 rows, running maximum, sum), which the combine kernel folds in the order of the runs.
+#pragma once
+
+#include "common.cuh"
+
+namespace lrqk {
+namespace tree {
+
+struct Params {
+  const void *q, *cache_k, *cache_v, *tree_k, *tree_v;
+  int64_t q_stride[3], ck_stride[3], cv_stride[3], tk_stride[3], tv_stride[3];
+  const int32_t *lens;      // [batch] or null: all `capacity` rows
+  const uint8_t *mask;      // [nodes][nodes] bytes per sequence, or null: node i sees nodes 0..i
+  int64_t mask_stride;      // between sequences
+  void *out;                // dense [batch][q_heads][nodes][head_dim]
+  float *lse;               // dense [batch][q_heads][nodes] or null
+  int32_t *status;          // device word that takes LRQK_ETIMEOUT, or null
+  float *part;              // partial rows: [slot][rows_per_block][head_dim], slot = (group * 2 + which) * row_blocks + block
+  float2 *part_ml;          // [slot][rows_per_block]: maximum (base-2 logarithm units), sum
+  float scale_log2;         // scale * log2(e)
+  int32_t batch, nodes, q_heads, cache_heads, tree_heads, head_dim, capacity;
+  int32_t rows;             // query rows of a unit: q_heads / cache_heads * nodes
+  int32_t rows_per_block, row_blocks, groups, tile_keys, tree_tiles;
+};
+
+__device__ __forceinline__ int cache_len(const Params &p, int b) {
+  if (!p.lens) return p.capacity;
+  return min(max(p.lens[b], 0), p.capacity);      // a length outside the cache is cut to it
+}
+__device__ __forceinline__ int cache_tiles(const Params &p, int len) { return (len + p.tile_keys - 1) / p.tile_keys; }
+
+// First tile of group g of `total` tiles; the group that holds tile x.
+__device__ __forceinline__ int64_t group_start(const Params &p, int64_t total, int g) { return total * g / p.groups; }
+__device__ __forceinline__ int group_of(const Params &p, int64_t total, int64_t x) { return (int)(((x + 1) * p.groups - 1) / total); }
+
+// One warp: the tiles of all units of the sequences before `upto`, and of all sequences.
+__device__ __forceinline__ void count_tiles(const Params &p, int upto, int64_t &before, int64_t &total) {
+  const int lane = threadIdx.x & 31;
+  int64_t s = 0, t = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    const int64_t n = (int64_t)p.cache_heads * (cache_tiles(p, cache_len(p, b)) + p.tree_tiles);
+    t += n;
+    if (b < upto) s += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+  }
+  before = s;
+  total = t;
+}
+
+// One warp: the sequence that tile x belongs to and the first tile of that sequence.
+__device__ __forceinline__ void find_sequence(const Params &p, int64_t x, int &seq, int64_t &base) {
+  const int lane = threadIdx.x & 31;
+  int64_t run = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int64_t n = b < p.batch ? (int64_t)p.cache_heads * (cache_tiles(p, cache_len(p, b)) + p.tree_tiles) : 0;
+    int64_t sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const unsigned hit = __ballot_sync(0xFFFFFFFFu, b < p.batch && run + sum > x);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      seq = b0 + l;
+      base = run + __shfl_sync(0xFFFFFFFFu, sum - n, l);
+      return;
+    }
+    run += __shfl_sync(0xFFFFFFFFu, sum, 31);
+  }
+  seq = p.batch;
+  base = run;
+}
+
+// The segments of one group's run: for (Walk w(...); w.valid(); w.next()).
+struct Walk {
+  int64_t x, end, base;     // next tile, end of the run, first tile of the sequence
+  int b, len, ctiles, per;  // sequence, its length, cache tiles and tiles per unit
+  int head, t0, t1;         // the segment: cache head, tiles [t0, t1) of the unit
+  bool first;               // the first segment of the run
+  __device__ __forceinline__ Walk(const Params &p, int64_t x0, int64_t x1, int seq, int64_t seq_base)
+      : x(x0), end(x1), base(seq_base), b(seq), first(true) {
+    if (x < end) { size(p); segment(); }
+  }
+  __device__ __forceinline__ void size(const Params &p) {
+    len = cache_len(p, b);
+    ctiles = cache_tiles(p, len);
+    per = ctiles + p.tree_tiles;
+  }
+  __device__ __forceinline__ void segment() {
+    const int64_t rel = x - base;
+    head = (int)(rel / per);
+    t0 = (int)(rel - (int64_t)head * per);
+    t1 = (int)min((int64_t)per, t0 + (end - x));
+  }
+  __device__ __forceinline__ bool valid() const { return x < end; }
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == per; }
+  __device__ __forceinline__ void next(const Params &p) {
+    x += t1 - t0;
+    first = false;
+    if (x >= end) return;
+    if (x - base >= (int64_t)per * p.cache_heads) {
+      base += (int64_t)per * p.cache_heads;
+      ++b;
+      size(p);
+    }
+    segment();
+  }
+  // where the partial of this segment goes: a run's first segment to slot 0, its last to slot 1
+  __device__ __forceinline__ int64_t slot(const Params &p, int group, int block) const {
+    return ((int64_t)group * 2 + (first ? 0 : 1)) * p.row_blocks + block;
+  }
+};
+
+// Does row `row` of the unit (node row % nodes) see drafted node j of sequence b?
+__device__ __forceinline__ bool sees(const Params &p, int b, int node, int j) {
+  return p.mask ? p.mask[b * p.mask_stride + (int64_t)node * p.nodes + j] != 0 : j <= node;
+}
+
+int launch_tc(const Params &p, cudaStream_t stream);     // bf16: tcgen05 kernel (tree_attention_tc.cu)
+bool plan_tc(Params &p);
+
+}  // namespace tree
+}  // namespace lrqk
