@@ -424,6 +424,32 @@ size_t lrqk_tree_attention_workspace_bytes(const lrqk_tree_args *a);
 int lrqk_tree_attention(const lrqk_tree_args *a, void *workspace, lrqk_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Choice of tokens from logits (the reference's drivers decode greedily, tps_estimate.py:41-84): temperature, top-k,
+ * top-p, min-p and a given random number per row.
+ *   w_i = exp((l_i - max) / T).  Top-k keeps the k largest logits, equal ones from the lowest index; of those top-p keeps, in
+ *   descending order, each token whose predecessors' mass is below p times the mass of all; of those min-p keeps w_i >=
+ *   min_p (relative to the largest).  The token is the first kept one, in index order, at which the cumulative mass exceeds
+ *   u times the kept mass.  Sums are whole numbers of 2^-44: the same token whatever the batch, the cluster or the order.
+ *   logits [rows, vocab] with row_stride elements between rows; u device fp32 [rows] in [0, 1); temperature, top_k,
+ *   top_p, min_p: device arrays [rows], or NULL to use the *_all value.  T = 0 (or negative): the first maximum.  top_k <= 0,
+ *   top_p >= 1, min_p <= 0 switch a filter off; the largest logit always stays.
+ *   tokens: out int64 [rows]; logprobs: optional out fp32 [rows], the logarithm of the token's share of the kept mass.
+ *   NaN counts as -inf; logits of +inf share the mass among themselves; a row of nothing but -inf and NaN gives -1, NaN.
+ *   vocab up to 409600 (fp32) or 819200 (bf16).  No workspace.
+ * ---------------------------------------------------------------------------------- */
+typedef struct lrqk_sample_args {
+  int32_t dtype, rows, vocab, top_k_all;
+  float temperature_all, top_p_all, min_p_all;
+  const void *logits;
+  int64_t row_stride;
+  const float *u, *temperature, *top_p, *min_p;
+  const int32_t *top_k;
+  int64_t *tokens;
+  float *logprobs;
+} lrqk_sample_args;
+int lrqk_sample_tokens(const lrqk_sample_args *a, lrqk_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * Element-wise glue of a decoder layer around the attention call, for the decode step (one token per
  * sequence), where every eager framework op is one launch of pure latency.  The reference leaves these to
  * the transformers modules (LlamaRMSNorm / Qwen2RMSNorm / MistralRMSNorm forward, the residual adds of the

@@ -38,8 +38,10 @@ from .extras import (  # noqa: F401,E402
 
 from .rotary import apply_rotary, rotary_frequencies  # noqa: F401,E402
 from .tree import check_tree_status, tree_attention, tree_mask  # noqa: F401,E402
+from .sampling import sample_tokens  # noqa: F401,E402
 
 __all__ = [
+    "sample_tokens",
     "check_tree_status", "tree_attention", "tree_mask",
     "apply_rotary", "rotary_frequencies",
     "FullOffloadCache", "HitRateCounter", "LightAttentionIndicesOffloadPrefill", "WrapForwardTimer", "run_task",

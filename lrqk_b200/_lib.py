@@ -90,6 +90,16 @@ class TreeArgs(C.Structure):
     ]
 
 
+class SampleArgs(C.Structure):
+    """struct lrqk_sample_args."""
+    _fields_ = [
+        ("dtype", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32), ("top_k_all", C.c_int32),
+        ("temperature_all", C.c_float), ("top_p_all", C.c_float), ("min_p_all", C.c_float),
+        ("logits", C.c_void_p), ("row_stride", C.c_int64), ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_p", C.c_void_p),
+        ("min_p", C.c_void_p), ("top_k", C.c_void_p), ("tokens", C.c_void_p), ("logprobs", C.c_void_p),
+    ]
+
+
 _SIGNATURES = {
     # name: (restype, argtypes)
     "lrqk_version": (C.c_char_p, []),
@@ -148,6 +158,7 @@ _SIGNATURES = {
     "lrqk_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
     "lrqk_tree_attention_workspace_bytes": (C.c_size_t, [C.POINTER(TreeArgs)]),
     "lrqk_tree_attention": (C.c_int, [C.POINTER(TreeArgs), C.c_void_p, C.c_void_p]),
+    "lrqk_sample_tokens": (C.c_int, [C.POINTER(SampleArgs), C.c_void_p]),
     "lrqk_add_rmsnorm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_float, C.c_int32, C.c_int32, C.c_int32,
                                    C.c_void_p, C.c_void_p, C.c_void_p]),
     "lrqk_swiglu": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
