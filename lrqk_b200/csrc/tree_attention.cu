@@ -19,12 +19,13 @@ template <int D> struct SimtShared {
   float q[kRows][D], k[kKeys][D + 4], v[kKeys][D], w[kRows][kKeys + 1];
 };
 
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_constant__ Params p) {
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   SimtShared<D> &sm = *reinterpret_cast<SimtShared<D> *>(smem_raw);
+  using T = float;
   constexpr int VE = Elt<T>::kPerVec, DC = D / 64;      // columns of a thread: DC runs of four
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int group = blockIdx.x / p.row_blocks, block = blockIdx.x % p.row_blocks;
@@ -231,9 +232,9 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   if (p.lse && lane == 0) p.lse[row] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
-template <typename T, int D> int launch_simt(const Params &p, cudaStream_t stream) {
+template <int D> int launch_simt(const Params &p, cudaStream_t stream) {
   static SmemOptIn opt_in;
-  auto kern = tree_simt_kernel<T, D>;
+  auto kern = tree_simt_kernel<D>;
   LRQK_CUDA_TRY(opt_in.ensure(kern, sizeof(SimtShared<D>)));
   LRQK_CUDA_TRY(launch_dependent(kern, dim3((unsigned)(p.groups * p.row_blocks)), dim3(kThreads), sizeof(SimtShared<D>), stream, 0, p));
   return LRQK_OK;
@@ -257,12 +258,16 @@ int plan(const lrqk_tree_args *a, Params &p) {
   p.batch = a->batch; p.nodes = a->nodes; p.q_heads = a->q_heads; p.cache_heads = a->cache_heads; p.tree_heads = a->tree_heads;
   p.head_dim = a->head_dim; p.capacity = (int32_t)a->capacity;
   p.rows = a->q_heads / a->cache_heads * a->nodes;
-  p.rows_per_block = kRows;
-  p.tile_keys = kKeys;
-  p.row_blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
-  // two CTAs an SM; the row blocks of a unit walk the same keys at the same time, so those are read from HBM once
-  p.groups = 2 * kNumSMs / p.row_blocks;
-  if (p.groups < 1) return LRQK_EUNSUPPORTED;
+  // The row blocks of a unit walk the same keys at the same time, so those come from HBM once.
+  if (a->dtype == LRQK_BF16) {
+    if (!plan_tc(p)) return LRQK_EUNSUPPORTED;
+  } else {
+    p.rows_per_block = kRows;
+    p.tile_keys = kKeys;
+    p.row_blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
+    p.groups = 2 * kNumSMs / p.row_blocks;   // two CTAs an SM
+    if (p.groups < 1) return LRQK_EUNSUPPORTED;
+  }
   p.tree_tiles = (p.nodes + p.tile_keys - 1) / p.tile_keys;
   return LRQK_OK;
 }
@@ -317,11 +322,10 @@ int lrqk_tree_attention(const lrqk_tree_args *a, void *workspace, lrqk_stream_t 
   p.part = static_cast<float *>(workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part + (size_t)p.groups * 2 * p.row_blocks * p.rows_per_block * p.head_dim);
   const cudaStream_t s = as_stream(stream);
-  LRQK_DISPATCH_DTYPE(a->dtype, T, {
-    rc = a->head_dim == 64 ? tree::launch_simt<T, 64>(p, s) : tree::launch_simt<T, 128>(p, s);
-    if (rc != LRQK_OK) return rc;
-    return a->head_dim == 64 ? tree::launch_combine<T, 64>(p, s) : tree::launch_combine<T, 128>(p, s);
-  });
+  if (a->dtype == LRQK_BF16) rc = tree::launch_tc(p, s);
+  else rc = a->head_dim == 64 ? tree::launch_simt<64>(p, s) : tree::launch_simt<128>(p, s);
+  if (rc != LRQK_OK) return rc;
+  LRQK_DISPATCH_DTYPE(a->dtype, T, return a->head_dim == 64 ? tree::launch_combine<T, 64>(p, s) : tree::launch_combine<T, 128>(p, s));
 }
 
 }  // extern "C"
