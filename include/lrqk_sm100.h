@@ -405,7 +405,7 @@ int lrqk_rotary(const lrqk_rotary_args *a, lrqk_stream_t stream);
  *                logarithm of the sum of exponentials.  A row that sees nothing gives zeros and -infinity.
  *   status     : optional device int32, zero before the first call: takes LRQK_ETIMEOUT if a bounded wait ran out; as
  *                long as it is set, calls hand out NaN rows.
- *   head_dim 64 or 128, up to 256 nodes.  The workspace needs no initialisation.
+ *   head_dim 64 or 128, up to 256 nodes.  out and workspace start on 32 bytes; the workspace needs no initialisation.
  * ---------------------------------------------------------------------------------- */
 typedef struct lrqk_tree_args {
   int32_t dtype, batch, nodes, q_heads, cache_heads, tree_heads, head_dim;

@@ -187,8 +187,8 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   const int per_head = p.q_heads / p.cache_heads, head = h / per_head;
   int64_t before, total;
   count_tiles(p, b, before, total);
-  const int per = cache_tiles(p, cache_len(p, b)) + p.tree_tiles;
-  const int64_t u0 = before + (int64_t)head * per;
+  const int ctiles = cache_tiles(p, cache_len(p, b)), per = ctiles + p.tree_tiles;
+  const int64_t u0 = before + (int64_t)head * unit_span(p, ctiles);
   const int g0 = group_of(p, total, u0), g1 = group_of(p, total, u0 + per - 1);
   if (g0 == g1) return;                                 // one run holds the unit: it is written already
   const int r = (h - head * per_head) * p.nodes + t, block = r / p.rows_per_block, at = r % p.rows_per_block;
@@ -216,14 +216,24 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
 #pragma unroll
     for (int c = 0; c < E; ++c) acc[c] *= fade;
     const int n = min(32, g1 - first + 1);
-    for (int i = 0; i < n; ++i) {
-      const float wi = __shfl_sync(0xFFFFFFFFu, weight, i), si = __shfl_sync(0xFFFFFFFFu, ml.y, i);
-      const int64_t at_i = __shfl_sync(0xFFFFFFFFu, slot, i);
-      if (si == 0.0f) continue;                         // nothing seen there (or no tiles)
-      sum = fmaf(wi, si, sum);
-      const float *src = p.part + at_i * D + lane * E;
+    for (int i = 0; i < n; i += 4) {                    // four runs' loads in flight
+      float part[4][E], wi[4], si[4];
 #pragma unroll
-      for (int c = 0; c < E; ++c) acc[c] = fmaf(wi, src[c], acc[c]);
+      for (int k = 0; k < 4; ++k) {
+        wi[k] = __shfl_sync(0xFFFFFFFFu, weight, (i + k) & 31);
+        si[k] = i + k < n ? __shfl_sync(0xFFFFFFFFu, ml.y, (i + k) & 31) : 0.0f;
+        const int64_t at_k = __shfl_sync(0xFFFFFFFFu, slot, (i + k) & 31);
+        const float *src = p.part + at_k * D + lane * E;
+#pragma unroll
+        for (int c = 0; c < E; ++c) part[k][c] = si[k] != 0.0f ? src[c] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (si[k] == 0.0f) continue;                    // nothing seen there (or no tiles)
+        sum = fmaf(wi[k], si[k], sum);
+#pragma unroll
+        for (int c = 0; c < E; ++c) acc[c] = fmaf(wi[k], part[k][c], acc[c]);
+      }
     }
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -258,12 +268,15 @@ int plan(const lrqk_tree_args *a, Params &p) {
   p.batch = a->batch; p.nodes = a->nodes; p.q_heads = a->q_heads; p.cache_heads = a->cache_heads; p.tree_heads = a->tree_heads;
   p.head_dim = a->head_dim; p.capacity = (int32_t)a->capacity;
   p.rows = a->q_heads / a->cache_heads * a->nodes;
+  p.per_node = 1.0f / (float)a->nodes;
+  if ((int64_t)a->q_heads / a->cache_heads * a->nodes > 1 << 16) return LRQK_EUNSUPPORTED;
   // The row blocks of a unit walk the same keys at the same time, so those come from HBM once.
   if (a->dtype == LRQK_BF16) {
     if (!plan_tc(p)) return LRQK_EUNSUPPORTED;
   } else {
     p.rows_per_block = kRows;
     p.tile_keys = kKeys;
+    p.unit_cost = 1;
     p.row_blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
     p.groups = 2 * kNumSMs / p.row_blocks;   // two CTAs an SM
     if (p.groups < 1) return LRQK_EUNSUPPORTED;
@@ -314,7 +327,7 @@ int lrqk_tree_attention(const lrqk_tree_args *a, void *workspace, lrqk_stream_t 
     if (a->q_stride[i] < 0 || a->tree_k_stride[i] < 0 || a->tree_v_stride[i] < 0 || a->cache_k_stride[i] < 0 || a->cache_v_stride[i] < 0)
       return LRQK_EINVAL;
   }
-  if (low & 15) return LRQK_EUNSUPPORTED;
+  if (low & 15 || (reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(workspace)) & 31) return LRQK_EUNSUPPORTED;
   p.q = a->q; p.cache_k = a->cache_k; p.cache_v = a->cache_v; p.tree_k = a->tree_k; p.tree_v = a->tree_v;
   p.lens = a->cache_lens; p.mask = a->mask; p.mask_stride = a->mask_stride;
   p.out = a->out; p.lse = a->lse; p.status = a->status;

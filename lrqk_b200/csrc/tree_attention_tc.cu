@@ -3,16 +3,19 @@
 //
 // A CTA walks its run of 128-key tiles with one or two blocks of 128 query rows (MT).  Per tile and row block
 //     S = Q K^T   tcgen05.mma M128 N128, K from a TMA tile (K-major), S in TMEM
-//     P = 2^(S c - m)   four warps, a thread per row: no exchange between lanes for the maximum and the sum
-//     O += P V    tcgen05.mma with P read from TMEM and V from its TMA tile (N = head_dim, MN-major), O in TMEM
-// P enters the product as TWO bf16 parts, high and low, over the columns of S that it replaces: rounding it to one bf16
-// would add as much error as the final rounding of the result; the second product hides behind the loads.
+//     P = 2^(S c - m)   two threads per row, 64 keys each
+//     O += P V    tcgen05.mma with P read from TMEM and V from its TMA tile (N = head_dim, MN-major), O in TMEM; in two halves
+// One row block: S has two buffers, the scores run a tile ahead.  P enters the product as TWO bf16 parts, high and low, over
+// the columns of S that it replaces: one bf16 would add as much error as the final rounding of the result, and the extra
+// product hides behind the loads (per tile 1536 of the 2800 cycles that HBM needs).
+// Two row blocks: 512 columns of TMEM hold two O and one S buffer each, one block's products run while the other's
+// weights are formed, and P is ONE bf16: with two parts the products alone would take 3072 of those 2800 cycles.
 // The running maximum moves only when a row's maximum has grown by more than 2^8 (then O is read, scaled and written
 // back by the row's thread); weights then stay below 2^8 and sums keep fp32's full precision.
 //
-// Warp 0 issues the copies (a ring of K and V tiles, 128-byte swizzle), warp 1 owns TMEM and issues the MMAs, warps 2.. are
-// four softmax warps per row block.  With one row block S is double-buffered, with two they alternate: while one
-// block's weights are formed, the other's products run.
+// Warp 0 issues the copies (a ring of K and V tiles, 128-byte swizzle), warp 1 owns TMEM and issues the products, warps
+// 2.. form the weights: a warp has 32 rows and one half of a tile's keys.  The maximum in use of a row passes from one half
+// to the next (of this tile, of the next one): each adds its own keys' before it forms its weights.
 //
 // V rows behind a length may hold anything, and 0 * NaN is NaN: the softmax warps clear them in shared memory before the
 // product.  In a drafted tile, values of V out of range are replaced by zeros and their nodes noted; a row that sees such
@@ -31,51 +34,101 @@ using namespace tc;
 
 constexpr int kTileKeys = 128, kBlockRows = 128;
 constexpr float kGrow = 8.0f;     // octaves a maximum may grow before O is rescaled
+constexpr int kOCol = 256;        // TMEM columns: S 0..255, O 256 + 128 * row block
 
 template <int D, int MT> struct Shape {
   static constexpr int kTileBytes = kTileKeys * D * 2;
   static constexpr int kHalfBytes = kTileKeys * 128;                 // 64 columns of a tile
   static constexpr int kQBytes = MT * kBlockRows * D * 2;
   static constexpr int kStages = (208 * 1024 - kQBytes) / kTileBytes > 8 ? 8 : (208 * 1024 - kQBytes) / kTileBytes;
-  static constexpr int kThreads = 64 + 128 * MT;
-  static constexpr int kBufs = MT == 1 ? 2 : 1;                      // S buffers of a row block
-  static constexpr int kOCol = 256;                                  // S: columns 0..255, O: 256 + 128 * block
+  static constexpr int kThreads = 64 + 256 * MT;
   static constexpr size_t kSmem = kQBytes + (size_t)kStages * kTileBytes + 1024;
 };
 
 struct Barriers {
-  uint64_t full[8], empty[8], s_full[2], p_ready[2], o_done[2], q_full;
+  uint64_t full[8], empty[8], q_full;
+  // [S buffer (one row block) or row block (two)], and the half of the keys
+  uint64_t s_full[2], p_ready[2][2], o_done[2][2];
+  uint64_t decided[2][2][4], pair[2][4];    // [row block][half][32 rows]: the maximum in use is set; [row block][32 rows]
+  float top[2][kBlockRows], sum[2][2][kBlockRows];
   uint32_t tmem, give_up, odd[2][4];        // odd: drafted rows of V with values out of range, 128 bits for each drafted tile
   int64_t x0, x1, base;
   int32_t seq;
 };
+
+// Bounded wait for a phase, suspended for up to 20 us a look: spinning on plain looks, the product warp alone issued 900
+// instructions a step and slowed the two softmax warps beside it by half.
+constexpr uint32_t kLooks = 1u << 17;       // a few seconds
+__device__ __forceinline__ bool await(uint64_t *bar, uint32_t parity) {
+  const uint32_t a = saddr(bar);
+  for (uint32_t i = 0; i < kLooks; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(a), "r"(parity), "r"(20000u) : "memory");
+    if (done) return true;
+  }
+  return false;
+}
 
 __device__ __forceinline__ void tma_tile(const CUtensorMap *map, void *dst, uint64_t *bar, int c0, int row, int head, int seq) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
                ::"r"(saddr(dst)), "l"(map), "r"(saddr(bar)), "r"(c0), "r"(row), "r"(head), "r"(seq) : "memory");
 }
 
-// D[tmem] (+)= A[tmem, 16-bit pairs in 32-bit columns] * B[shared]
-__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one;
+}
+// Products issued by the lane whose `leader` is 1; all lanes of the warp come along.
+// D[tmem] (+)= A[shared] * B[shared]
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+// D[tmem] (+)= A[tmem, 16-bit pairs in 32-bit columns] * B[shared]
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar, uint32_t leader) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+               "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(saddr(bar)), "r"(leader) : "memory");
 }
 
-// 32 columns of this warp's lanes; the wait names the registers, so that no use can move ahead of it
-__device__ __forceinline__ void load32(uint32_t taddr, uint32_t (&v)[32]) {
+// 32 columns of this warp's lanes.  The registers are defined once pin() has followed the wait.
+__device__ __forceinline__ void load32_async(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      "\n\ttcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
         "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
         "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// An empty statement behind the wait that names the registers, so that no use can move ahead of it.
+__device__ __forceinline__ void pin(uint32_t (&v)[32]) {
+  asm volatile("" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                    "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]));
+  asm volatile("" : "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
+                    "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
+__device__ __forceinline__ void load32(uint32_t taddr, uint32_t (&v)[32]) {
+  load32_async(taddr, v);
+  load_wait();
+  pin(v);
 }
 __device__ __forceinline__ void store32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
@@ -88,6 +141,10 @@ __device__ __forceinline__ void store32(uint32_t taddr, const uint32_t (&v)[32])
         "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]),
         "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void store8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+               ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -99,6 +156,81 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Eight columns of O times a row's factor.
+__device__ __forceinline__ void scale8(uint32_t taddr, float f) {
+  uint32_t v[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]) : "r"(taddr) : "memory");
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * f);
+  store8(taddr, v);
+}
+
+// Pairs of fp32 in one register pair: one instruction for two multiply-adds.
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) { return ((uint64_t)b << 32) | a; }
+__device__ __forceinline__ uint64_t pair(float a, float b) { return pair(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float low_of(uint64_t a) { return __uint_as_float((uint32_t)a); }
+__device__ __forceinline__ float high_of(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Weights of 32 keys of a row, 2^(s c - m), in the place of their scores; adds to the sums.
+__device__ __forceinline__ void weigh(uint32_t (&s)[32], uint64_t c2, uint64_t minus2, uint64_t &sum2) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 2) {
+    const uint64_t x = fma2(pair(s[j], s[j + 1]), c2, minus2);
+    const float a = exp2_fast(low_of(x)), b = exp2_fast(high_of(x));
+    sum2 = add2(sum2, pair(a, b));
+    s[j] = __float_as_uint(a);
+    s[j + 1] = __float_as_uint(b);
+  }
+}
+// ... as bf16: high parts into 16 columns, low parts into the next 16
+__device__ __forceinline__ void store_two_parts(const uint32_t (&w)[32], uint32_t taddr) {
+  const uint64_t less = pair(-1.0f, -1.0f);
+  uint32_t o[32];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    o[j] = pack_bf16(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+    const uint64_t rest = fma2(pair(o[j] << 16, o[j] & 0xFFFF0000u), less, pair(w[2 * j], w[2 * j + 1]));
+    o[16 + j] = pack_bf16(low_of(rest), high_of(rest));
+  }
+  store32(taddr, o);
+}
+__device__ __forceinline__ float max32(const uint32_t (&s)[32]) {
+  float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < 32; j += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) part[k] = max3(part[k], __uint_as_float(s[j + 2 * k]), __uint_as_float(s[j + 2 * k + 1]));
+  return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+
+// Scores of keys that the row does not see: minus infinity.
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t seen) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[j] = (seen >> j) & 1u ? s[j] : 0xFF800000u;
+}
+
+// 32 bytes of a row (a thread's own row: whole sectors, half the instructions of 16-byte stores)
+__device__ __forceinline__ void st32(void *dst, const uint32_t *v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
 struct Maps { CUtensorMap ck, cv, tk, tv; };
@@ -120,8 +252,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) { mbar_init(&bar.full[i], 1); mbar_init(&bar.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_ready[i], 128); mbar_init(&bar.o_done[i], 1); }
-    mbar_init(&bar.q_full, 128 * MT);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1);
+    for (int i = 0; i < 4; ++i) { mbar_init(&bar.p_ready[i >> 1][i & 1], 4); mbar_init(&bar.o_done[i >> 1][i & 1], 1); }
+    for (int i = 0; i < 16; ++i) mbar_init(&bar.decided[i >> 3][(i >> 2) & 1][i & 3], 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&bar.pair[i >> 2][i & 3], 2);
+    mbar_init(&bar.q_full, 8 * MT);
     bar.give_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -163,7 +298,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           const int row = (drafted ? t - w.ctiles : t) * kTileKeys;
           for (int v = 0; v < 2; ++v, ++i) {
             const int s = i % S::kStages;
-            if (i >= S::kStages && !wait_bounded(&bar.empty[s], (i / S::kStages - 1) & 1)) { quit(); break; }
+            if (i >= S::kStages && !await(&bar.empty[s], (i / S::kStages - 1) & 1)) { quit(); break; }
             const CUtensorMap *m = drafted ? (v ? &maps.tv : &maps.tk) : (v ? &maps.cv : &maps.ck);
             const int head = drafted ? tree_head * (v ? co.tv_head : co.tk_head) : w.head * (v ? co.cv_head : co.ck_head);
             const int seq = w.b * (drafted ? (v ? co.tv_seq : co.tk_seq) : (v ? co.cv_seq : co.ck_seq));
@@ -176,209 +311,198 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       }
     }
   } else if (warp == 1) {
-    // ---- products ------------------------------------------------------------------------------------------------------
-    if (lane == 0) {
-      constexpr uint32_t kIdescS = umma_idesc_bf16_k(128, kTileKeys);
-      constexpr uint32_t kIdescO = umma_idesc_bf16_k(128, D) | (1u << 16);       // B (the values) MN-major
-      const uint32_t q_base = saddr(qs), stage_base = saddr(stages);
-      const auto scores = [&](int i, int m, int buf) {
-        const uint32_t kb = stage_base + (uint32_t)(i % S::kStages) * S::kTileBytes, qb = q_base + m * (kBlockRows * D * 2);
+    // ---- products: the whole warp walks along, so that descriptors stay in uniform registers; one lane issues ----------------
+    constexpr uint32_t kIdescS = umma_idesc_bf16_k(128, kTileKeys);
+    constexpr uint32_t kIdescO = umma_idesc_bf16_k(128, D) | (1u << 16);       // B (the values) MN-major
+    const uint32_t leader = elect_one();
+    const uint64_t q_desc = umma_desc_k_sw128(saddr(qs), 1024), k_desc = umma_desc_k_sw128(saddr(stages), 1024);
+    const uint64_t v_desc = umma_desc_mn_sw128(saddr(stages), S::kHalfBytes, 1024);
+    const auto ready = [&](uint64_t *b, uint32_t parity) {
+      if (__all_sync(0xFFFFFFFFu, await(b, parity))) { fence_after(); return true; }
+      quit();
+      return false;
+    };
+    // (Addresses in descriptors count 16 bytes.)  `i`: ring index of the tile; x: its scores' buffer.
+    const auto scores = [&](int i, int m, int x) {
+      const uint64_t kd = k_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes) >> 4), qd = q_desc + (uint64_t)(m * ((kBlockRows * D * 2) >> 4));
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * S::kHalfBytes + (ks & 3) * 32;
-          umma_bf16(tmem + buf * 128, umma_desc_k_sw128(qb + off, 1024), umma_desc_k_sw128(kb + off, 1024), kIdescS, ks > 0);
-        }
-        umma_commit(&bar.s_full[buf]);
-      };
-      const auto values = [&](int i, int m, int buf, bool fresh) {
-        const uint32_t vb = stage_base + (uint32_t)(i % S::kStages) * S::kTileBytes;
-#pragma unroll
-        for (int ks = 0; ks < kTileKeys / 16; ++ks) {
-          const uint64_t desc = umma_desc_mn_sw128(vb + ks * 2048, S::kHalfBytes, 1024);
-          const uint32_t a = tmem + buf * 128 + (ks >> 1) * 32 + (ks & 1) * 8;   // high parts; low parts 16 columns on
-          umma_bf16_ts(tmem + S::kOCol + m * 128, a, desc, kIdescO, !(fresh && ks == 0));
-          umma_bf16_ts(tmem + S::kOCol + m * 128, a + 16, desc, kIdescO, 1);
-        }
-        umma_commit(&bar.o_done[m]);
-      };
-      const auto arrived = [&](int i) {
-        if (wait_bounded(&bar.full[i % S::kStages], (i / S::kStages) & 1)) { fence_after(); return true; }
-        quit();
-        return false;
-      };
-      int i = 0, cnt = 0, seg = 0;         // ring index of the next tile's K, tiles done, segments done
-      for (; w.valid() && !*give_up; w.next(p), ++seg) {
-        const int n = w.t1 - w.t0;
-        if (!wait_bounded(&bar.q_full, seg & 1)) { quit(); break; }
-        fence_after();
-        if (!arrived(i)) break;
-        if constexpr (MT == 1) {
-          scores(i, 0, cnt & 1);
-          umma_commit(&bar.empty[i % S::kStages]);
-          for (int t = 0; t < n; ++t, ++cnt, i += 2) {
-            if (t + 1 < n) {
-              if (!arrived(i + 2)) break;
-              scores(i + 2, 0, (cnt + 1) & 1);
-              umma_commit(&bar.empty[(i + 2) % S::kStages]);
-            }
-            if (!arrived(i + 1)) break;
-            if (!wait_bounded(&bar.p_ready[cnt & 1], (cnt >> 1) & 1)) { quit(); break; }
-            fence_after();
-            values(i + 1, 0, cnt & 1, t == 0);
-            umma_commit(&bar.empty[(i + 1) % S::kStages]);
-          }
-        } else {
-          scores(i, 0, 0);
-          scores(i, 1, 1);
-          umma_commit(&bar.empty[i % S::kStages]);
-          for (int t = 0; t < n; ++t, ++cnt, i += 2) {
-            if (!arrived(i + 1)) break;
-            bool ok = true;
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              if (!wait_bounded(&bar.p_ready[m], cnt & 1)) { quit(); ok = false; break; }
-              fence_after();
-              values(i + 1, m, m, t == 0);
-              if (m == 1) umma_commit(&bar.empty[(i + 1) % S::kStages]);
-              if (t + 1 < n) {
-                if (m == 0 && !arrived(i + 2)) { ok = false; break; }
-                scores(i + 2, m, m);
-                if (m == 1) umma_commit(&bar.empty[(i + 2) % S::kStages]);
-              }
-            }
-            if (!ok) break;
-          }
-        }
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint64_t off = ((ks >> 2) * S::kHalfBytes + (ks & 3) * 32) >> 4;
+        umma_ss(tmem + x * 128, qd + off, kd + off, kIdescS, ks > 0, leader);
       }
+      commit(&bar.s_full[x], leader);
+    };
+    // the product with the values, each half of the keys as soon as its weights are there
+    const auto values = [&](int i, int m, int x, uint32_t parity, bool fresh) {
+      const uint32_t d = tmem + kOCol + m * 128;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!ready(&bar.p_ready[x][half], parity)) return false;
+        const uint64_t vd = v_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes + half * 64 * 128) >> 4);
+        const uint32_t a = tmem + x * 128 + half * 64;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const bool add = !(fresh && half == 0 && ks == 0);
+          if constexpr (MT == 1) {         // per 32 keys: 16 columns of high parts, 16 of low parts
+            const uint32_t at = a + (ks >> 1) * 32 + (ks & 1) * 8;
+            umma_ts(d, at, vd + ks * (2048 >> 4), kIdescO, add, leader);
+            umma_ts(d, at + 16, vd + ks * (2048 >> 4), kIdescO, 1, leader);
+          } else {
+            umma_ts(d, a + ks * 8, vd + ks * (2048 >> 4), kIdescO, add, leader);
+          }
+        }
+        commit(&bar.o_done[x][half], leader);
+      }
+      return true;
+    };
+    const auto arrived = [&](int i) { return ready(&bar.full[i % S::kStages], (i / S::kStages) & 1); };
+    const auto release = [&](int i) { commit(&bar.empty[i % S::kStages], leader); };
+    int i = 0, cnt = 0, seg = 0;           // ring index of the tile's K, tiles done, segments done
+    for (; w.valid() && !*give_up; w.next(p), ++seg) {
+      const int n = w.t1 - w.t0;
+      bool ok = ready(&bar.q_full, seg & 1) && arrived(i);
+      if (!ok) break;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) scores(i, m, MT == 1 ? cnt & 1 : m);
+      release(i);
+      for (int t = 0; t < n; ++t, ++cnt, i += 2) {
+        const bool more = t + 1 < n;
+        if constexpr (MT == 1) {
+          if (more) {
+            if (!(ok = arrived(i + 2))) break;
+            scores(i + 2, 0, (cnt + 1) & 1);
+            release(i + 2);
+          }
+          if (!(ok = arrived(i + 1) && values(i + 1, 0, cnt & 1, (cnt >> 1) & 1, t == 0))) break;
+        } else {
+          if (!(ok = arrived(i + 1) && values(i + 1, 0, 0, cnt & 1, t == 0))) break;
+          if (more) {
+            if (!(ok = arrived(i + 2))) break;
+            scores(i + 2, 0, 0);
+          }
+          if (!(ok = values(i + 1, 1, 1, cnt & 1, t == 0))) break;
+          if (more) {
+            scores(i + 2, 1, 1);
+            release(i + 2);
+          }
+        }
+        release(i + 1);
+      }
+      if (!ok) break;
     }
   } else {
-    // ---- softmax: a thread per query row ---------------------------------------------------------------------------------
-    const int m = (warp - 2) >> 2;                       // row block of this warp
+    // ---- weights: two threads per query row, 64 keys of a tile each ----------------------------------------------------------
+    const int m = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1;                             // row block, half of the keys
     const int quarter = warp & 3, r_in = quarter * 32 + lane, row = m * kBlockRows + r_in;   // TMEM lanes 32 * (warp % 4)..
-    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), o_base = lane_base + S::kOCol + m * 128;
-    const int at_row = row0 + row, g = at_row / p.nodes, node = at_row % p.nodes;            // query head in the group, node
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), o_base = lane_base + kOCol + m * 128;
+    const int g = group_row(p, row0 + row), node = row0 + row - g * p.nodes;                // query head in the group, node
     const bool real = row < n_rows, warp_real = m * kBlockRows + quarter * 32 < n_rows;
-    int cnt = 0, i = 0;
-    for (; w.valid() && !*give_up; w.next(p)) {
-      // the block's queries, into the K-major swizzled operand (rows that do not exist: zeros)
+    int cnt = 0, i0 = 0, seg = 0;                        // tiles done, ring index of the segment's first K, segments done
+    const auto signal = [&](uint64_t *b) {               // one arrival for the warp, behind all of its lanes' writes
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b);
+    };
+    for (; w.valid() && !*give_up; w.next(p), ++seg) {
+      // the block's queries, for the K-major swizzled operand (rows that do not exist: zeros); all loads in flight at once
+      constexpr int kLoaders = 256, kLoads = kBlockRows * (D / 8) / kLoaders;
+      uint4 qv[kLoads];
       {
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + w.b * p.q_stride[0] + (int64_t)(w.head * per_head) * p.q_stride[1];
-        unsigned char *dst = qs + m * (kBlockRows * D * 2);
-        const int t128 = quarter * 32 + lane;
-        for (int e = t128; e < kBlockRows * (D / 8); e += 128) {
-          const int r = e / (D / 8), c = e % (D / 8), ar = row0 + m * kBlockRows + r;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (m * kBlockRows + r < n_rows) v = ld16(q + (int64_t)(ar / p.nodes) * p.q_stride[1] + (int64_t)(ar % p.nodes) * p.q_stride[2] + c * 8);
-          *reinterpret_cast<uint4 *>(dst + (c >> 3) * (kBlockRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&bar.q_full);
-      }
-      // which nodes of the segment's first drafted tile this row sees
-      uint32_t seen[4] = {0, 0, 0, 0};
-      int seen_tile = -1;
-      const auto look = [&](int dt) {
-        seen_tile = dt;
-        const int first = dt * kTileKeys, n = min(kTileKeys, p.nodes - first);
+        const int first = half * 128 + quarter * 32 + lane;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t bits = 0;
-          if (real)
-            for (int j = 0; j < 32 && c * 32 + j < n; ++j) bits |= (sees(p, w.b, node, first + c * 32 + j) ? 1u : 0u) << j;
-          seen[c] = bits;
+        for (int k = 0; k < kLoads; ++k) {
+          const int e = first + k * kLoaders, r = m * kBlockRows + e / (D / 8), c = e % (D / 8);
+          const int gr = group_row(p, row0 + r);
+          qv[k] = make_uint4(0, 0, 0, 0);
+          if (r < n_rows) qv[k] = ld16(q + gr * p.q_stride[1] + (int64_t)(row0 + r - gr * p.nodes) * p.q_stride[2] + c * 8);
+        }
+      }
+      // which nodes of a drafted step this row sees
+      uint32_t seen[2] = {0, 0};
+      int seen_at = -1;
+      const auto look = [&](int at) {                    // a row of the mask at a time, a lane per node: coalesced, no exchange
+        seen_at = at;
+        const uint8_t *mask = p.mask ? p.mask + w.b * p.mask_stride : nullptr;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int first = at + c * 32, j = first + lane;
+          seen[c] = 0;
+          if (first >= p.nodes) continue;
+          if (!mask) {
+            const int n = node - first;                  // nodes up to its own
+            seen[c] = n >= 31 ? 0xFFFFFFFFu : n >= 0 ? (2u << n) - 1u : 0u;
+            continue;
+          }
+#pragma unroll 16
+          for (int r = 0; r < 32; ++r) {
+            const int other = __shfl_sync(0xFFFFFFFFu, node, r);
+            const bool yes = j < p.nodes && mask[(int64_t)other * p.nodes + j] != 0;
+            const uint32_t word = __ballot_sync(0xFFFFFFFFu, yes);
+            if (lane == r) seen[c] = word;
+          }
         }
       };
-      if (w.t1 > w.ctiles) look(max(w.t0 - w.ctiles, 0));
-      float top = -INFINITY, sum = 0.0f;                 // maximum in use, in octaves; sum of weights
-      for (int t = w.t0; t < w.t1; ++t, ++cnt, i += 2) {
-        const int buf = MT == 1 ? (cnt & 1) : m;
-        const uint32_t s_base = lane_base + buf * 128;
-        const bool drafted = t >= w.ctiles;
-        const int dt = t - w.ctiles, n_keys = min(kTileKeys, drafted ? p.nodes - dt * kTileKeys : w.len - t * kTileKeys);
-        if (drafted && dt != seen_tile) look(dt);
-        if (!wait_bounded(&bar.s_full[buf], MT == 1 ? (cnt >> 1) & 1 : cnt & 1)) { quit(); break; }
-        fence_after();
-        bool waited = t == w.t0;                         // for the products of the tile before
-        if (warp_real) {
-          const bool all = !drafted && n_keys == kTileKeys;
-          uint32_t v[32];
-          float big = -INFINITY;
+      if (warp_real && w.t1 > w.ctiles) look(max(w.t0 - w.ctiles, 0) * kTileKeys + half * 64);   // ahead of its use
+      {
+        unsigned char *dst = qs + m * (kBlockRows * D * 2);
+        const int first = half * 128 + quarter * 32 + lane;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            load32(s_base + c * 32, v);
-            if (all) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) big = fmaxf(big, __uint_as_float(v[j]));
-            } else {
-              const uint32_t bits = drafted ? seen[c] : (n_keys >= c * 32 + 32 ? 0xFFFFFFFFu : n_keys > c * 32 ? (1u << (n_keys - c * 32)) - 1u : 0u);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) big = fmaxf(big, (bits >> j) & 1u ? __uint_as_float(v[j]) : -INFINITY);
-            }
-          }
-          const float now = big * p.scale_log2;
-          const bool move = now > top + kGrow || (top == -INFINITY && now > -INFINITY);
-          if (__any_sync(0xFFFFFFFFu, move)) {
-            const float fade = move ? exp2_fast(top - now) : 1.0f;
-            if (move) { sum *= fade; top = now; }
-            if (!waited) {
-              if (!wait_bounded(&bar.o_done[m], (cnt - 1) & 1)) { quit(); break; }
-              fence_after();
-              waited = true;
-#pragma unroll
-              for (int c = 0; c < D; c += 32) {
-                load32(o_base + c, v);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * fade);
-                store32(o_base + c, v);
-              }
-            }
-          }
-          const float minus = top == -INFINITY ? 0.0f : -top;
-          float add0 = 0.0f, add1 = 0.0f;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            load32(s_base + c * 32, v);
-            const uint32_t bits = all ? 0xFFFFFFFFu : drafted ? seen[c] : (n_keys >= c * 32 + 32 ? 0xFFFFFFFFu : n_keys > c * 32 ? (1u << (n_keys - c * 32)) - 1u : 0u);
-            uint32_t o[32];
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              float a = exp2_fast(fmaf(__uint_as_float(v[j]), p.scale_log2, minus)), b = exp2_fast(fmaf(__uint_as_float(v[j + 1]), p.scale_log2, minus));
-              if (!all) {
-                a = (bits >> j) & 1u ? a : 0.0f;
-                b = (bits >> (j + 1)) & 1u ? b : 0.0f;
-              }
-              add0 += a;
-              add1 += b;
-              const uint32_t hi = pack_bf16(a, b);
-              o[j >> 1] = hi;
-              o[16 + (j >> 1)] = pack_bf16(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xFFFF0000u));
-            }
-            store32(s_base + c * 32, o);
-          }
-          sum += add0 + add1;
+        for (int k = 0; k < kLoads; ++k) {
+          const int e = first + k * kLoaders, r = e / (D / 8), c = e % (D / 8);
+          *reinterpret_cast<uint4 *>(dst + (c >> 3) * (kBlockRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = qv[k];
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        signal(&bar.q_full);
+      }
+      float top = -INFINITY, sum = 0.0f;                 // maximum in use, in octaves; sum of this thread's weights
+      const int n_tiles = w.t1 - w.t0, plain = w.len / kTileKeys - w.t0;   // the first `plain` tiles are seen whole
+      for (int st = 0; st < n_tiles; ++st, ++cnt) {
+        const int x = MT == 1 ? cnt & 1 : m;
+        const uint32_t parity = MT == 1 ? (cnt >> 1) & 1 : cnt & 1;
+        const uint32_t s_base = lane_base + x * 128 + half * 64;
+        const bool masked = st >= plain;
+        int n_keys = kTileKeys, dt = -1;                 // filled keys of the tile; drafted tile
+        if (masked) {
+          dt = w.t0 + st - w.ctiles;
+          n_keys = min(kTileKeys, dt >= 0 ? p.nodes - dt * kTileKeys : w.len - (w.t0 + st) * kTileKeys);
+          if (warp_real && dt >= 0 && dt * kTileKeys + half * 64 != seen_at) look(dt * kTileKeys + half * 64);
+        }
+        const bool drafted = dt >= 0;
+        if (!await(&bar.s_full[x], parity)) { quit(); break; }
+        fence_after();
         // values that must not meet the product: rows of the cache behind the length, drafted rows out of range
-        if (m == 0 && (drafted || n_keys < kTileKeys)) {
+        if (masked && m == 0 && half == 0) {
+          const int i = i0 + 2 * st;
           const int vi = (i + 1) % S::kStages;
           unsigned char *vt = stages + (size_t)vi * S::kTileBytes;
-          if (!wait_bounded(&bar.full[vi], ((i + 1) / S::kStages) & 1)) { quit(); break; }
-          const bool behind = r_in >= n_keys;
+          if (!await(&bar.full[vi], ((i + 1) / S::kStages) & 1)) { quit(); break; }
+          // this thread's row of the tile, 16 bytes at a time (in an order that keeps the banks apart)
+          const auto piece = [&](int c) { return reinterpret_cast<uint4 *>(vt + (c >> 3) * S::kHalfBytes + r_in * 128 + (((c + lane) & 7) << 4)); };
           bool odd = false;
-          for (int c = 0; c < D / 8; ++c) {
-            uint4 *at = reinterpret_cast<uint4 *>(vt + (c >> 3) * S::kHalfBytes + r_in * 128 + (((c + lane) & 7) << 4));
-            if (behind) {
-              *at = make_uint4(0, 0, 0, 0);
-            } else if (drafted) {
-              const uint4 x = *at;
-              uint32_t y[4] = {x.x, x.y, x.z, x.w};
-              bool here = false;
+          if (r_in >= n_keys) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {              // exponent of all ones: infinite or not a number
-                if ((y[e] & 0x7F80u) == 0x7F80u) { y[e] &= 0xFFFF0000u; here = true; }
-                if ((y[e] & 0x7F800000u) == 0x7F800000u) { y[e] &= 0x0000FFFFu; here = true; }
+            for (int c = 0; c < D / 8; ++c) *piece(c) = make_uint4(0, 0, 0, 0);
+          } else if (drafted) {
+            uint32_t most = 0;                           // largest magnitude, as two 16-bit patterns
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+              const uint4 y = *piece(c);
+              most = __vmaxu2(__vmaxu2(most, y.x & 0x7FFF7FFFu), y.y & 0x7FFF7FFFu);
+              most = __vmaxu2(__vmaxu2(most, y.z & 0x7FFF7FFFu), y.w & 0x7FFF7FFFu);
+            }
+            odd = (most & 0xFFFFu) >= 0x7F80u || (most >> 16) >= 0x7F80u;   // exponent of all ones: infinite or not a number
+            if (odd) {
+#pragma unroll 1
+              for (int c = 0; c < D / 8; ++c) {
+                const uint4 y4 = *piece(c);
+                uint32_t y[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if ((y[e] & 0x7F80u) == 0x7F80u) y[e] &= 0xFFFF0000u;
+                  if ((y[e] & 0x7F800000u) == 0x7F800000u) y[e] &= 0x0000FFFFu;
+                }
+                *piece(c) = make_uint4(y[0], y[1], y[2], y[3]);
               }
-              if (here) *at = make_uint4(y[0], y[1], y[2], y[3]);
-              odd |= here;
             }
           }
           if (drafted) {
@@ -387,16 +511,83 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        if (!waited && !wait_bounded(&bar.o_done[m], (cnt - 1) & 1)) { quit(); break; }
+        if (warp_real) {
+          uint32_t v[32], u[32];
+          load32_async(s_base, v);
+          load32_async(s_base + 32, u);
+          load_wait();
+          pin(v);
+          pin(u);
+          if (masked) {
+            const int n = n_keys - half * 64;            // filled keys of this half
+            hide(v, drafted ? seen[0] : n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u);
+            hide(u, drafted ? seen[1] : n >= 64 ? 0xFFFFFFFFu : n > 32 ? (1u << (n - 32)) - 1u : 0u);
+          }
+          const float now = fmaxf(max32(v), max32(u)) * p.scale_log2;
+          // the maximum in use, from the half before
+          float old = top;
+          if (half == 1 || cnt > 0) {
+            if (!await(&bar.decided[m][half ^ 1][quarter], (half == 1 ? cnt : cnt - 1) & 1)) { quit(); break; }
+            if (half == 1 || st > 0) top = bar.top[m][r_in];
+          }
+          const bool move = now > top + kGrow || (top == -INFINITY && now > -INFINITY);
+          const float use = move ? now : top;
+          if (move || (half == 0 && st == 0)) bar.top[m][r_in] = use;
+          signal(&bar.decided[m][half][quarter]);
+          if (__any_sync(0xFFFFFFFFu, move) && (half == 1 || st > 0)) {
+            // O holds the products up to the half before: that one has to be in it
+            const int px = MT == 1 ? (half == 1 ? x : x ^ 1) : m, pc = half == 1 ? cnt : cnt - 1;
+            if (!await(&bar.o_done[px][half ^ 1], (MT == 1 ? pc >> 1 : pc) & 1)) { quit(); break; }
+            fence_after();
+            const float fade = move ? exp2_fast(top - use) : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 8) scale8(o_base + c, fade);
+          }
+          top = use;
+          if (old != top) sum *= exp2_fast(old - top);
+          const uint64_t c2 = pair(p.scale_log2, p.scale_log2), minus2 = top == -INFINITY ? 0 : pair(-top, -top);
+          uint64_t sum2 = 0;
+          weigh(v, c2, minus2, sum2);
+          if constexpr (MT == 1) {
+            store_two_parts(v, s_base);
+            weigh(u, c2, minus2, sum2);
+            store_two_parts(u, s_base + 32);
+          } else {
+            weigh(u, c2, minus2, sum2);
+            uint32_t o[32];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              o[j] = pack_bf16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+              o[16 + j] = pack_bf16(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+            }
+            store32(s_base, o);
+          }
+          sum += low_of(sum2) + high_of(sum2);
+        }
         store_wait();
         fence_before();
-        mbar_arrive(&bar.p_ready[buf]);
+        signal(&bar.p_ready[x][half]);
       }
+      i0 += 2 * n_tiles;
       if (*give_up) break;
-      if (!wait_bounded(&bar.o_done[m], (cnt - 1) & 1)) { quit(); break; }
-      fence_after();
-      // ---- the segment's rows: finished, or a partial ------------------------------------------------------------------
+      {
+        const int x = MT == 1 ? (cnt - 1) & 1 : m;
+        if (!await(&bar.o_done[x][1], (MT == 1 ? (cnt - 1) >> 1 : cnt - 1) & 1)) { quit(); break; }
+        fence_after();
+      }
+      // ---- the segment's rows: finished, or a partial; a row's threads share its columns ------------------------------------
       if (warp_real) {
+        if (half == 0) {                                 // the maximum that the last half set
+          if (!await(&bar.decided[m][1][quarter], (cnt - 1) & 1)) { quit(); break; }
+          const float last = bar.top[m][r_in];
+          if (last != top) sum *= exp2_fast(top - last);
+          top = last;
+        }
+        bar.sum[m][half][r_in] = sum;
+        signal(&bar.pair[m][quarter]);
+        if (!await(&bar.pair[m][quarter], seg & 1)) { quit(); break; }
+        sum += bar.sum[m][half ^ 1][r_in];
+        constexpr int kCols = D / 2;
         const bool whole = w.whole();
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int64_t at = ((int64_t)w.b * p.q_heads + w.head * per_head + g) * p.nodes + node;
@@ -405,7 +596,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         if (w.t1 > w.ctiles)
           for (int c = 0; c < 8; ++c) any_odd |= *reinterpret_cast<volatile uint32_t *>(&bar.odd[c >> 2][c & 3]);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
+        for (int cc = 0; cc < kCols; cc += 32) {
+          const int c = half * kCols + cc;
           uint32_t v[32];
           load32(o_base + c, v);
           if (any_odd && real) {
@@ -414,6 +606,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
               for (int j = dt * kTileKeys; j < min(p.nodes, (dt + 1) * kTileKeys); ++j) {
                 if (!((*reinterpret_cast<volatile uint32_t *>(&bar.odd[dt & 1][(j & 127) >> 5]) >> (j & 31)) & 1u) || !sees(p, w.b, node, j)) continue;
                 const __nv_bfloat16 *src = static_cast<const __nv_bfloat16 *>(p.tree_v) + w.b * p.tv_stride[0] + (w.head / share) * p.tv_stride[1] + j * p.tv_stride[2] + c;
+#pragma unroll
                 for (int e = 0; e < 32; ++e) {
                   const float x = __bfloat162float(src[e]);
                   if (!(fabsf(x) < INFINITY)) v[e] = __float_as_uint(__uint_as_float(v[e]) + x);
@@ -422,22 +615,22 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           }
           if (real) {
             if (whole) {
-              uint4 *dst = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.out) + at * D + c);
+              __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(p.out) + at * D + c;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                uint32_t o[4];
+              for (int e = 0; e < 2; ++e) {
+                uint32_t o[8];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[k] = pack_bf16(__uint_as_float(v[8 * e + 2 * k]) * inv, __uint_as_float(v[8 * e + 2 * k + 1]) * inv);
-                dst[e] = make_uint4(o[0], o[1], o[2], o[3]);
+                for (int k = 0; k < 8; ++k) o[k] = pack_bf16(__uint_as_float(v[16 * e + 2 * k]) * inv, __uint_as_float(v[16 * e + 2 * k + 1]) * inv);
+                st32(dst + 16 * e, o);
               }
             } else {
-              uint4 *dst = reinterpret_cast<uint4 *>(p.part + slot * D + c);
+              float *dst = p.part + slot * D + c;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) dst[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+              for (int e = 0; e < 4; ++e) st32(dst + 8 * e, v + 8 * e);
             }
           }
         }
-        if (real) {
+        if (real && half == 0) {
           if (!whole) p.part_ml[slot] = make_float2(top, sum);
           else if (p.lse) p.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
         }
@@ -497,6 +690,7 @@ template <int D, int MT> int launch(const Params &p, cudaStream_t stream) {
 bool plan_tc(Params &p) {
   p.rows_per_block = p.rows <= kBlockRows ? kBlockRows : 2 * kBlockRows;
   p.tile_keys = kTileKeys;
+  p.unit_cost = 4;
   p.row_blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
   p.groups = kNumSMs / p.row_blocks;
   return p.groups >= 1;

@@ -3,8 +3,11 @@
 // A unit is one (sequence, cache head) and one block of its query rows (rows = the G query heads that read the cache
 // head, times the nodes).  Its keys come in tiles: first the filled rows of the cache, then the drafted nodes.  All units'
 // tiles, laid end to end, are cut into `groups` equal runs, one per CTA, whatever the sequences' lengths are; those are read
-// on the device, so a captured call follows them.  A unit that falls into several runs leaves one partial result per
-// run (fp32 rows, running maximum, sum), which the combine kernel folds in the order of the runs.
+// on the device, so a captured call follows them.  Starting and ending a unit (its queries, its mask, its rows) takes a CTA as
+// long as a few tiles, so `unit_cost` empty tiles stand behind each unit's own: without them the CTA that got the
+// shortest sequences' units, nine of them beside twelve tiles elsewhere, ran three times as long as the others.
+// A unit that falls into several runs leaves one partial result per run (fp32 rows, running maximum, sum), which the combine
+// kernel folds in the order of the runs.
 #pragma once
 
 #include "common.cuh"
@@ -24,9 +27,10 @@ struct Params {
   float *part;              // partial rows: [slot][rows_per_block][head_dim], slot = (group * 2 + which) * row_blocks + block
   float2 *part_ml;          // [slot][rows_per_block]: maximum (base-2 logarithm units), sum
   float scale_log2;         // scale * log2(e)
+  float per_node;           // 1 / nodes
   int32_t batch, nodes, q_heads, cache_heads, tree_heads, head_dim, capacity;
   int32_t rows;             // query rows of a unit: q_heads / cache_heads * nodes
-  int32_t rows_per_block, row_blocks, groups, tile_keys, tree_tiles;
+  int32_t rows_per_block, row_blocks, groups, tile_keys, tree_tiles, unit_cost;
 };
 
 __device__ __forceinline__ int cache_len(const Params &p, int b) {
@@ -34,6 +38,7 @@ __device__ __forceinline__ int cache_len(const Params &p, int b) {
   return min(max(p.lens[b], 0), p.capacity);      // a length outside the cache is cut to it
 }
 __device__ __forceinline__ int cache_tiles(const Params &p, int len) { return (len + p.tile_keys - 1) / p.tile_keys; }
+__device__ __forceinline__ int unit_span(const Params &p, int ctiles) { return ctiles + p.tree_tiles + p.unit_cost; }
 
 // First tile of group g of `total` tiles; the group that holds tile x.
 __device__ __forceinline__ int64_t group_start(const Params &p, int64_t total, int g) { return total * g / p.groups; }
@@ -44,7 +49,7 @@ __device__ __forceinline__ void count_tiles(const Params &p, int upto, int64_t &
   const int lane = threadIdx.x & 31;
   int64_t s = 0, t = 0;
   for (int b = lane; b < p.batch; b += 32) {
-    const int64_t n = (int64_t)p.cache_heads * (cache_tiles(p, cache_len(p, b)) + p.tree_tiles);
+    const int64_t n = (int64_t)p.cache_heads * unit_span(p, cache_tiles(p, cache_len(p, b)));
     t += n;
     if (b < upto) s += n;
   }
@@ -63,7 +68,7 @@ __device__ __forceinline__ void find_sequence(const Params &p, int64_t x, int &s
   int64_t run = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     const int b = b0 + lane;
-    const int64_t n = b < p.batch ? (int64_t)p.cache_heads * (cache_tiles(p, cache_len(p, b)) + p.tree_tiles) : 0;
+    const int64_t n = b < p.batch ? (int64_t)p.cache_heads * unit_span(p, cache_tiles(p, cache_len(p, b))) : 0;
     int64_t sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -83,45 +88,50 @@ __device__ __forceinline__ void find_sequence(const Params &p, int64_t x, int &s
   base = run;
 }
 
-// The segments of one group's run: for (Walk w(...); w.valid(); w.next()).
+// The segments of one group's run [x0, x1): for (Walk w(...); w.valid(); w.next(p)).
 struct Walk {
-  int64_t x, end, base;     // next tile, end of the run, first tile of the sequence
-  int b, len, ctiles, per;  // sequence, its length, cache tiles and tiles per unit
-  int head, t0, t1;         // the segment: cache head, tiles [t0, t1) of the unit
-  bool first;               // the first segment of the run
-  __device__ __forceinline__ Walk(const Params &p, int64_t x0, int64_t x1, int seq, int64_t seq_base)
-      : x(x0), end(x1), base(seq_base), b(seq), first(true) {
-    if (x < end) { size(p); segment(); }
+  int64_t x0, end, base, unit;   // the run; first tile of the sequence, of the unit
+  int b, len, ctiles, per;       // sequence, its length, cache tiles and own tiles of a unit
+  int head, t0, t1;              // the segment: cache head, tiles [t0, t1) of the unit
+  __device__ __forceinline__ Walk(const Params &p, int64_t run0, int64_t run1, int seq, int64_t seq_base)
+      : x0(run0), end(run1), base(seq_base), b(seq) {
+    if (x0 >= end) { unit = end; return; }
+    size(p);
+    const int span = unit_span(p, ctiles);
+    head = (int)((x0 - base) / span);
+    unit = base + (int64_t)head * span;
+    t0 = (int)(x0 - unit);
+    t1 = (int)min((int64_t)per, end - unit);
+    if (t0 >= per) next(p);      // the run starts on empty tiles
   }
   __device__ __forceinline__ void size(const Params &p) {
     len = cache_len(p, b);
     ctiles = cache_tiles(p, len);
     per = ctiles + p.tree_tiles;
   }
-  __device__ __forceinline__ void segment() {
-    const int64_t rel = x - base;
-    head = (int)(rel / per);
-    t0 = (int)(rel - (int64_t)head * per);
-    t1 = (int)min((int64_t)per, t0 + (end - x));
-  }
-  __device__ __forceinline__ bool valid() const { return x < end; }
+  __device__ __forceinline__ bool valid() const { return unit < end; }
   __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == per; }
   __device__ __forceinline__ void next(const Params &p) {
-    x += t1 - t0;
-    first = false;
-    if (x >= end) return;
-    if (x - base >= (int64_t)per * p.cache_heads) {
-      base += (int64_t)per * p.cache_heads;
+    unit += unit_span(p, ctiles);
+    if (unit >= end) return;
+    if (++head == p.cache_heads) {
+      head = 0;
+      base = unit;
       ++b;
       size(p);
     }
-    segment();
+    t0 = 0;
+    t1 = (int)min((int64_t)per, end - unit);
   }
-  // where the partial of this segment goes: a run's first segment to slot 0, its last to slot 1
+  // where the partial of this segment goes: to slot 0 for the unit that the run starts in, to slot 1 for the one it ends in
   __device__ __forceinline__ int64_t slot(const Params &p, int group, int block) const {
-    return ((int64_t)group * 2 + (first ? 0 : 1)) * p.row_blocks + block;
+    return ((int64_t)group * 2 + (x0 >= unit ? 0 : 1)) * p.row_blocks + block;
   }
 };
+
+// row / nodes for a row of a unit, without an integer division: below 2^16 rows the product is within 2^-6 / nodes of
+// (row + 1/2) / nodes, which lies half of 1 / nodes from a whole number.
+__device__ __forceinline__ int group_row(const Params &p, int row) { return (int)(((float)row + 0.5f) * p.per_node); }
 
 // Does row `row` of the unit (node row % nodes) see drafted node j of sequence b?
 __device__ __forceinline__ bool sees(const Params &p, int b, int node, int j) {
