@@ -66,13 +66,18 @@ class PeerGroup(C.Structure):
     ]
 
 
+def _three(name):
+    """An int64_t[3] of the C struct as three fields: a struct built from plain numbers is filled in one call."""
+    return [(f"{name}{i}", C.c_int64) for i in range(3)]
+
+
 class RotaryArgs(C.Structure):
     """struct lrqk_rotary_args."""
     _fields_ = [
         ("dtype", C.c_int32), ("batch", C.c_int32), ("length", C.c_int32), ("q_heads", C.c_int32), ("k_heads", C.c_int32),
         ("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("adjoint", C.c_int32),
-        ("positions_are_64bit", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p), ("q_stride", C.c_int64 * 3),
-        ("k_stride", C.c_int64 * 3), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("positions", C.c_void_p),
+        ("positions_are_64bit", C.c_int32), ("q", C.c_void_p), ("k", C.c_void_p), *_three("q_stride"),
+        *_three("k_stride"), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("positions", C.c_void_p),
         ("position_stride", C.c_int64), ("inv_freq", C.c_void_p), ("factor", C.c_float),
     ]
 
@@ -83,8 +88,7 @@ class TreeArgs(C.Structure):
         ("dtype", C.c_int32), ("batch", C.c_int32), ("nodes", C.c_int32), ("q_heads", C.c_int32), ("cache_heads", C.c_int32),
         ("tree_heads", C.c_int32), ("head_dim", C.c_int32), ("scale", C.c_float), ("capacity", C.c_int64),
         ("q", C.c_void_p), ("cache_k", C.c_void_p), ("cache_v", C.c_void_p), ("tree_k", C.c_void_p), ("tree_v", C.c_void_p),
-        ("q_stride", C.c_int64 * 3), ("cache_k_stride", C.c_int64 * 3), ("cache_v_stride", C.c_int64 * 3),
-        ("tree_k_stride", C.c_int64 * 3), ("tree_v_stride", C.c_int64 * 3),
+        *_three("q_stride"), *_three("cache_k_stride"), *_three("cache_v_stride"), *_three("tree_k_stride"), *_three("tree_v_stride"),
         ("cache_lens", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("out", C.c_void_p), ("lse", C.c_void_p),
         ("status", C.c_void_p),
     ]

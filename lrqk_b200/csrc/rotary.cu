@@ -205,8 +205,9 @@ extern "C" int lrqk_rotary(const lrqk_rotary_args *a, lrqk_stream_t stream) {
   uintptr_t low = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->q_out);
   if (a->k_heads) low |= reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->k_out);
   for (int i = 0; i < 3; ++i) {
-    p.stride[0][i] = a->q_stride[i];
-    p.stride[1][i] = a->k_heads ? a->k_stride[i] : 0;
+    const int32_t n[2][3] = {{a->batch, a->q_heads, a->length}, {a->batch, a->k_heads, a->length}};
+    p.stride[0][i] = n[0][i] > 1 ? a->q_stride[i] : 0;   // (a dimension with one entry has no stride that matters)
+    p.stride[1][i] = n[1][i] > 1 && a->k_heads ? a->k_stride[i] : 0;
     low |= (uintptr_t)((p.stride[0][i] | p.stride[1][i]) * (int64_t)elt_size(a->dtype));
   }
   p.positions = a->positions; p.pos_stride = a->position_stride; p.pos64 = a->positions_are_64bit;

@@ -315,17 +315,18 @@ int lrqk_tree_attention(const lrqk_tree_args *a, void *workspace, lrqk_stream_t 
   uintptr_t low = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->tree_k) | reinterpret_cast<uintptr_t>(a->tree_v) |
                   reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(workspace);
   if (a->capacity > 0) low |= reinterpret_cast<uintptr_t>(a->cache_k) | reinterpret_cast<uintptr_t>(a->cache_v);
-  for (int i = 0; i < 3; ++i) {
-    p.q_stride[i] = a->q_stride[i];
-    p.ck_stride[i] = a->cache_k_stride[i];
-    p.cv_stride[i] = a->cache_v_stride[i];
-    p.tk_stride[i] = a->tree_k_stride[i];
-    p.tv_stride[i] = a->tree_v_stride[i];
-    const int64_t all = a->q_stride[i] | a->tree_k_stride[i] | a->tree_v_stride[i] |
-                        (a->capacity > 0 ? a->cache_k_stride[i] | a->cache_v_stride[i] : 0);
-    low |= (uintptr_t)(all * (int64_t)elt_size(a->dtype));
-    if (a->q_stride[i] < 0 || a->tree_k_stride[i] < 0 || a->tree_v_stride[i] < 0 || a->cache_k_stride[i] < 0 || a->cache_v_stride[i] < 0)
-      return LRQK_EINVAL;
+  // (a dimension with one entry has no stride that matters)
+  const struct { const int64_t *from; int64_t *to; int32_t heads; int64_t rows; } tensors[5] = {
+      {a->q_stride, p.q_stride, a->q_heads, a->nodes}, {a->cache_k_stride, p.ck_stride, a->cache_heads, a->capacity},
+      {a->cache_v_stride, p.cv_stride, a->cache_heads, a->capacity}, {a->tree_k_stride, p.tk_stride, a->tree_heads, a->nodes},
+      {a->tree_v_stride, p.tv_stride, a->tree_heads, a->nodes}};
+  for (const auto &t : tensors) {
+    if (t.rows == 0) continue;
+    t.to[0] = a->batch > 1 ? t.from[0] : 0;
+    t.to[1] = t.heads > 1 ? t.from[1] : 0;
+    t.to[2] = t.rows > 1 ? t.from[2] : 0;
+    if (t.to[0] < 0 || t.to[1] < 0 || t.to[2] < 0) return LRQK_EINVAL;
+    low |= (uintptr_t)((t.to[0] | t.to[1] | t.to[2]) * (int64_t)elt_size(a->dtype));
   }
   if (low & 15 || (reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(workspace)) & 31) return LRQK_EUNSUPPORTED;
   p.q = a->q; p.cache_k = a->cache_k; p.cache_v = a->cache_v; p.tree_k = a->tree_k; p.tree_v = a->tree_v;

@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .state import _DTYPES, _stream, on_device
+from .state import _DTYPES, call_on
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, seq_len: Optional[int] = None,
@@ -82,38 +82,27 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
     return (inv if device is None else inv.to(device)), out
 
 
-def _check(x: torch.Tensor, name: str, like: Optional[torch.Tensor] = None):
-    if x.dim() != 4 or x.dtype not in _DTYPES or not x.is_cuda:
-        raise ValueError(f"{name}: expected a float32 or bfloat16 CUDA tensor [batch, heads, length, head_dim], got {x.dtype} "
-                         f"{tuple(x.shape)} on {x.device}")
-    if like is not None and (x.dtype != like.dtype or x.device != like.device or x.shape[0] != like.shape[0]
-                             or x.shape[2:] != like.shape[2:]):
-        raise ValueError(f"{name}: batch, length, head_dim, dtype and device must be those of q, got {x.dtype} {tuple(x.shape)} on {x.device}")
-
-
-def _dense_last(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
-
-
 def _rotate(q, k, positions, inv_freq, factor, interleaved, adjoint):
     b, hq, n, d = q.shape
-    q = _dense_last(q)
-    q_out = torch.empty((b, hq, n, d), dtype=q.dtype, device=q.device)
-    a = _lib.RotaryArgs()
-    a.dtype, a.batch, a.length, a.q_heads, a.head_dim = _DTYPES[q.dtype], b, n, hq, d
-    a.rotary_dim, a.interleaved, a.adjoint, a.factor = 2 * inv_freq.shape[0], interleaved, adjoint, factor
-    a.q, a.q_out, a.q_stride[:] = q.data_ptr(), q_out.data_ptr(), q.stride()[:3]
-    k_out = None
-    if k is not None:
-        k = _dense_last(k)
-        k_out = torch.empty((b, k.shape[1], n, d), dtype=q.dtype, device=q.device)
-        a.k_heads, a.k, a.k_out, a.k_stride[:] = k.shape[1], k.data_ptr(), k_out.data_ptr(), k.stride()[:3]
-    a.positions, a.positions_are_64bit = positions.data_ptr(), positions.dtype == torch.int64
-    a.position_stride = positions.stride(0) if positions.shape[0] > 1 else 0
-    a.inv_freq = inv_freq.data_ptr()
-    if q_out.numel():
-        with on_device(q.device):
-            _lib.check(_lib.lib().lrqk_rotary(a, _stream()), "lrqk_rotary")
+    qs = q.stride()
+    if qs[3] != 1 and d > 1:
+        q = q.contiguous()
+        qs = q.stride()
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is None:
+        hk, k_out, k_at, k_to, ks = 0, None, None, None, (0, 0, 0)
+    else:
+        ks = k.stride()
+        if ks[3] != 1 and d > 1:
+            k = k.contiguous()
+            ks = k.stride()
+        hk, k_out = k.shape[1], torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_at, k_to = k.data_ptr(), k_out.data_ptr()
+    if b and n:
+        a = _lib.RotaryArgs(_DTYPES[q.dtype], b, n, hq, hk, d, 2 * inv_freq.shape[0], interleaved, adjoint, positions.dtype is torch.int64,
+                            q.data_ptr(), k_at, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], q_out.data_ptr(), k_to, positions.data_ptr(),
+                            positions.stride(0) if positions.shape[0] > 1 else 0, inv_freq.data_ptr(), factor)
+        _lib.check(call_on(q.device, _lib.lib().lrqk_rotary, a), "lrqk_rotary")
     return q_out, k_out
 
 
@@ -147,20 +136,22 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
 
     Strided inputs (a transposed projection) are read as they are; the results are contiguous.  Differentiable in ``q`` and
     ``k``.  Returns ``(q', k')``, or ``q'`` when ``k`` is ``None``."""
-    _check(q, "q")
-    if k is not None:
-        _check(k, "k", q)
+    if q.dim() != 4 or q.dtype not in _DTYPES or not q.is_cuda:
+        raise ValueError(f"q: expected a float32 or bfloat16 CUDA tensor [batch, heads, length, head_dim], got {q.dtype} {tuple(q.shape)} on {q.device}")
     b, _, n, d = q.shape
-    if positions.dtype not in (torch.int64, torch.int32) or positions.device != q.device:
-        raise ValueError(f"positions: expected int64 or int32 on {q.device}, got {positions.dtype} on {positions.device}")
+    device = q.device
+    if k is not None and (k.dim() != 4 or k.dtype is not q.dtype or k.device != device or k.shape[0] != b or k.shape[2] != n or k.shape[3] != d):
+        raise ValueError(f"k: expected {q.dtype} [{b}, heads, {n}, {d}] on {device}, got {k.dtype} {tuple(k.shape)} on {k.device}")
+    if positions.dtype not in (torch.int64, torch.int32) or positions.device != device:
+        raise ValueError(f"positions: expected int64 or int32 on {device}, got {positions.dtype} on {positions.device}")
     if positions.dim() == 1:
         positions = positions.unsqueeze(0)
     if positions.dim() != 2 or positions.shape[1] != n or positions.shape[0] not in (1, b):
         raise ValueError(f"positions: expected [{n}], [1, {n}] or [{b}, {n}], got {tuple(positions.shape)}")
     if n > 1 and positions.stride(1) != 1:
         positions = positions.contiguous()
-    if inv_freq.dtype != torch.float64 or inv_freq.device != q.device or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq: expected a contiguous float64 vector on {q.device}, got {inv_freq.dtype} {tuple(inv_freq.shape)} "
+    if inv_freq.dtype is not torch.float64 or inv_freq.device != device or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq: expected a contiguous float64 vector on {device}, got {inv_freq.dtype} {tuple(inv_freq.shape)} "
                          f"on {inv_freq.device}")
     if not 0 < 2 * inv_freq.shape[0] <= d:
         raise ValueError(f"inv_freq: {inv_freq.shape[0]} pairs do not fit a head of {d}")

@@ -10,7 +10,7 @@ from typing import Tuple, Union
 import torch
 
 from . import _lib
-from .state import _DTYPES, _stream, on_device
+from .state import _DTYPES, call_on
 
 Setting = Union[float, int, torch.Tensor]
 
@@ -43,19 +43,17 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting
     rows, vocab = logits.shape
     if u.dtype != torch.float32 or u.device != logits.device or u.shape != (rows,) or not u.is_contiguous():
         raise ValueError(f"u: expected contiguous float32 [{rows}] on {logits.device}, got {u.dtype} {tuple(u.shape)} on {u.device}")
-    a = _lib.SampleArgs()
-    a.temperature, a.temperature_all = _setting(temperature, "temperature", rows, logits.device, torch.float32, 0.0)
-    a.top_k, a.top_k_all = _setting(top_k, "top_k", rows, logits.device, torch.int32, 0)
-    a.top_p, a.top_p_all = _setting(top_p, "top_p", rows, logits.device, torch.float32, 0.0)
-    a.min_p, a.min_p_all = _setting(min_p, "min_p", rows, logits.device, torch.float32, 0.0)
+    device = logits.device
+    t, t_all = _setting(temperature, "temperature", rows, device, torch.float32, 0.0)
+    k, k_all = _setting(top_k, "top_k", rows, device, torch.int32, 0)
+    p, p_all = _setting(top_p, "top_p", rows, device, torch.float32, 0.0)
+    m, m_all = _setting(min_p, "min_p", rows, device, torch.float32, 0.0)
     if logits.stride(1) != 1 and vocab > 1:
         logits = logits.contiguous()
-    tokens = torch.empty((rows,), dtype=torch.int64, device=logits.device)
-    logprobs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
-    if rows == 0:
-        return tokens, logprobs
-    a.dtype, a.rows, a.vocab, a.logits, a.row_stride = _DTYPES[logits.dtype], rows, vocab, logits.data_ptr(), logits.stride(0) if rows > 1 else 0
-    a.u, a.tokens, a.logprobs = u.data_ptr(), tokens.data_ptr(), logprobs.data_ptr()
-    with on_device(logits.device):
-        _lib.check(_lib.lib().lrqk_sample_tokens(a, _stream()), "lrqk_sample_tokens")
+    tokens = torch.empty((rows,), dtype=torch.int64, device=device)
+    logprobs = torch.empty_like(u)
+    if rows:
+        a = _lib.SampleArgs(_DTYPES[logits.dtype], rows, vocab, k_all, t_all, p_all, m_all, logits.data_ptr(), logits.stride(0) if rows > 1 else 0,
+                            u.data_ptr(), t, p, m, k, tokens.data_ptr(), logprobs.data_ptr())
+        _lib.check(call_on(device, _lib.lib().lrqk_sample_tokens, a), "lrqk_sample_tokens")
     return tokens, logprobs

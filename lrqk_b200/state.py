@@ -127,6 +127,19 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def call_on(device: torch.device, fn, *args) -> int:
+    """``fn(*args, stream)`` with the device's current stream, and with the device current: the short way for calls whose
+    host time counts (one look at the current device, the raw stream, no context object in the common case)."""
+    index = device.index
+    if _get_device() == index:
+        return fn(*args, _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(index):
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
 class LayerState:
     def __init__(self, bsz: int, q_heads: int, kv_heads: int, head_dim: int, r: int, k: int, m: int,
                  a_capacity: int, host_capacity: int, dtype: torch.dtype, device="cuda", max_iter: int = 2,

@@ -13,7 +13,7 @@ from typing import Dict, Optional, Sequence, Union
 import torch
 
 from . import _lib
-from .state import _DTYPES, _stream, on_device
+from .state import _DTYPES, call_on
 
 MAX_NODES = 256
 
@@ -64,21 +64,11 @@ def check_tree_status(device=None) -> None:
         raise _lib.LrqkError(code, "lrqk_tree_attention", _lib.lib().lrqk_strerror(code).decode())
 
 
-def _rows(x: torch.Tensor, name: str, q: torch.Tensor, rows: Optional[int]) -> torch.Tensor:
-    if x.dim() != 4 or x.dtype != q.dtype or x.device != q.device or x.shape[0] != q.shape[0] or x.shape[3] != q.shape[3] or \
-            (rows is not None and x.shape[2] != rows):
-        raise ValueError(f"{name}: expected {q.dtype} [{q.shape[0]}, heads, {'rows' if rows is None else rows}, {q.shape[3]}] on {q.device}, "
-                         f"got {x.dtype} {tuple(x.shape)} on {x.device}")
-    return x
-
-
-def _strides(x: torch.Tensor, name: str):
-    """(batch, head, row) strides; rows start on 16 bytes.  A dimension of one row has no stride that matters."""
-    s, e = x.stride(), x.element_size()
-    st = [0 if n == 1 else v for n, v in zip(x.shape[:3], s[:3])]
-    if (x.shape[3] > 1 and s[3] != 1) or x.data_ptr() % 16 or any(v * e % 16 for v in st):
-        raise ValueError(f"{name}: rows must be dense and start on 16 bytes; strides {tuple(s)} at address {x.data_ptr():#x}")
-    return st
+def _refuse_rows(**tensors):
+    for name, x in tensors.items():
+        s, e = x.stride(), x.element_size()
+        if x.numel() and (x.data_ptr() % 16 or any(n > 1 and v * e % 16 for n, v in zip(x.shape[:3], s))):
+            raise ValueError(f"{name}: rows must start on 16 bytes; strides {tuple(s)} at address {x.data_ptr():#x}")
 
 
 def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor, tree_k: torch.Tensor, tree_v: torch.Tensor,
@@ -101,14 +91,14 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     if q.dim() != 4 or q.dtype not in _DTYPES or not q.is_cuda:
         raise ValueError(f"q: expected a float32 or bfloat16 CUDA tensor [batch, heads, nodes, head_dim], got {q.dtype} {tuple(q.shape)} on {q.device}")
     b, hq, t, d = q.shape
-    _rows(cache_k, "cache_k", q, None)
-    _rows(cache_v, "cache_v", q, cache_k.shape[2])
-    _rows(tree_k, "tree_k", q, t)
-    _rows(tree_v, "tree_v", q, t)
-    hc, ht, cap = cache_k.shape[1], tree_k.shape[1], cache_k.shape[2]
-    if cache_v.shape[1] != hc or tree_v.shape[1] != ht or hc == 0 or ht == 0 or hq % hc or hc % ht or hq == 0:
-        raise ValueError(f"heads: keys and values alike, tree heads dividing cache heads dividing query heads; got q {hq}, "
-                         f"cache {hc} / {cache_v.shape[1]}, tree {ht} / {tree_v.shape[1]}")
+    device, dtype = q.device, q.dtype
+    hc, cap, ht = cache_k.shape[1], cache_k.shape[2], tree_k.shape[1]
+    for name, x, shape in (("cache_k", cache_k, (b, hc, cap, d)), ("cache_v", cache_v, (b, hc, cap, d)), ("tree_k", tree_k, (b, ht, t, d)),
+                           ("tree_v", tree_v, (b, ht, t, d))):
+        if x.shape != shape or x.dtype is not dtype or x.device != device:
+            raise ValueError(f"{name}: expected {dtype} {list(shape)} on {device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    if hc == 0 or ht == 0 or hq == 0 or hq % hc or hc % ht:
+        raise ValueError(f"heads: tree heads divide cache heads divide query heads; got q {hq}, cache {hc}, tree {ht}")
     if t > MAX_NODES:
         raise ValueError(f"at most {MAX_NODES} nodes, got {t}")
     if d not in (64, 128):
@@ -118,33 +108,35 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     scale = d ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    out = torch.empty((b, hq, t, d), dtype=q.dtype, device=q.device)
-    lse = torch.empty((b, hq, t), dtype=torch.float32, device=q.device) if return_lse else None
-    if out.numel() == 0:
-        return (out, lse) if return_lse else out
-    a = _lib.TreeArgs()
-    a.dtype, a.batch, a.nodes, a.q_heads, a.cache_heads, a.tree_heads, a.head_dim = _DTYPES[q.dtype], b, t, hq, hc, ht, d
-    a.scale, a.capacity = scale, cap
-    a.q, a.q_stride[:] = q.data_ptr(), _strides(q, "q")
-    if cap:
-        a.cache_k, a.cache_k_stride[:] = cache_k.data_ptr(), _strides(cache_k, "cache_k")
-        a.cache_v, a.cache_v_stride[:] = cache_v.data_ptr(), _strides(cache_v, "cache_v")
-    a.tree_k, a.tree_k_stride[:] = tree_k.data_ptr(), _strides(tree_k, "tree_k")
-    a.tree_v, a.tree_v_stride[:] = tree_v.data_ptr(), _strides(tree_v, "tree_v")
+    qs, ks, vs, tks, tvs = q.stride(), cache_k.stride(), cache_v.stride(), tree_k.stride(), tree_v.stride()
+    if not qs[3] == ks[3] == vs[3] == tks[3] == tvs[3] == 1:
+        raise ValueError("q, cache_k, cache_v, tree_k, tree_v: rows must be dense (last stride 1)")
+    mask_at = lens_at = lse_at = None
+    mask_stride = 0
     if mask is not None:
-        if mask.dtype not in (torch.bool, torch.uint8) or mask.device != q.device or mask.shape[-2:] != (t, t) or \
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.device != device or mask.shape[-2:] != (t, t) or \
                 not (mask.dim() == 2 or (mask.dim() == 3 and mask.shape[0] in (1, b))):
-            raise ValueError(f"mask: expected bool [{t}, {t}] or [{b}, {t}, {t}] on {q.device}, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
+            raise ValueError(f"mask: expected bool [{t}, {t}] or [{b}, {t}, {t}] on {device}, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
         mask = mask.contiguous()
-        a.mask, a.mask_stride = mask.data_ptr(), t * t if mask.dim() == 3 and mask.shape[0] > 1 else 0
+        mask_at, mask_stride = mask.data_ptr(), t * t if mask.dim() == 3 and mask.shape[0] > 1 else 0
     if cache_lens is not None:
-        if cache_lens.dtype != torch.int32 or cache_lens.device != q.device or cache_lens.shape != (b,) or not cache_lens.is_contiguous():
-            raise ValueError(f"cache_lens: expected contiguous int32 [{b}] on {q.device}, got {cache_lens.dtype} {tuple(cache_lens.shape)} on {cache_lens.device}")
-        a.cache_lens = cache_lens.data_ptr()
-    a.out, a.lse = out.data_ptr(), None if lse is None else lse.data_ptr()
-    lib = _lib.lib()
-    with on_device(q.device):
-        a.status = _status_word(q.device)
-        ws = torch.empty((lib.lrqk_tree_attention_workspace_bytes(a),), dtype=torch.uint8, device=q.device)
-        _lib.check(lib.lrqk_tree_attention(a, ws.data_ptr(), _stream()), "lrqk_tree_attention")
+        if cache_lens.dtype is not torch.int32 or cache_lens.device != device or cache_lens.shape != (b,) or not cache_lens.is_contiguous():
+            raise ValueError(f"cache_lens: expected contiguous int32 [{b}] on {device}, got {cache_lens.dtype} {tuple(cache_lens.shape)} on {cache_lens.device}")
+        lens_at = cache_lens.data_ptr()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = None
+    if return_lse:
+        lse = torch.empty((b, hq, t), dtype=torch.float32, device=device)
+        lse_at = lse.data_ptr()
+    if b and t:
+        lib = _lib.lib()
+        a = _lib.TreeArgs(_DTYPES[dtype], b, t, hq, hc, ht, d, scale, cap, q.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(),
+                          tree_k.data_ptr(), tree_v.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                          tks[0], tks[1], tks[2], tvs[0], tvs[1], tvs[2], lens_at, mask_at, mask_stride, out.data_ptr(), lse_at,
+                          _status_word(device))
+        ws = torch.empty((lib.lrqk_tree_attention_workspace_bytes(a),), dtype=torch.uint8, device=device)
+        code = call_on(device, lib.lrqk_tree_attention, a, ws.data_ptr())
+        if code == _lib.EUNSUPPORTED:
+            _refuse_rows(q=q, cache_k=cache_k, cache_v=cache_v, tree_k=tree_k, tree_v=tree_v)
+        _lib.check(code, "lrqk_tree_attention")
     return (out, lse) if return_lse else out
