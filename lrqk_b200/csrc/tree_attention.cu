@@ -29,11 +29,9 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
   constexpr int VE = Elt<T>::kPerVec, DC = D / 64;      // columns of a thread: DC runs of four
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const int group = blockIdx.x / p.row_blocks, block = blockIdx.x % p.row_blocks;
-  int64_t before, total;
-  count_tiles(p, 0, before, total);
-  const int64_t x0 = group_start(p, total, group), x1 = group_start(p, total, group + 1);
-  int seq = 0;
-  int64_t base = 0;
+  const Cut cut(p, count_tiles(p, 0).total);
+  const int x0 = cut.start(group), x1 = cut.start(group + 1);
+  int seq = 0, base = 0;
   if (x0 < x1) find_sequence(p, x0, seq, base);
   const int row0 = block * kRows, n_rows = min(kRows, p.rows - row0), per_head = p.q_heads / p.cache_heads;
   const bool works = ty * 4 < n_rows;                   // rows of this thread exist
@@ -171,39 +169,34 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
 // One warp per query row of a unit that was cut: the row's partials, folded in the order of the runs.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Params p) {
-  pdl_launch_dependents();
-  pdl_wait();
   constexpr int E = D / 32;                             // columns of a lane
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= (int64_t)p.batch * p.q_heads * p.nodes) return;
-  const int t = (int)(row % p.nodes), h = (int)(row / p.nodes % p.q_heads), b = (int)(row / p.nodes / p.q_heads);
-  T *dst = static_cast<T *>(p.out) + row * D + lane * E;
-  if (p.status && *reinterpret_cast<volatile int32_t *>(p.status) != 0) {   // a wait ran out: no row can be trusted
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);  // (batch * q_heads * nodes is below 2^31)
+  if (row >= p.batch * p.q_heads * p.nodes) return;
+  const int t = row % p.nodes, h = row / p.nodes % p.q_heads, b = row / p.nodes / p.q_heads;
+  const int32_t broken = p.status ? *reinterpret_cast<volatile int32_t *>(p.status) : 0;
+  const Count n = count_tiles(p, b);
+  T *dst = static_cast<T *>(p.out) + (int64_t)row * D + lane * E;
+  if (broken != 0) {                                    // a wait ran out: no row can be trusted
     for (int c = 0; c < E; ++c) dst[c] = Elt<T>::from_float(NAN);
     if (p.lse && lane == 0) p.lse[row] = NAN;
     return;
   }
   const int per_head = p.q_heads / p.cache_heads, head = h / per_head;
-  int64_t before, total;
-  count_tiles(p, b, before, total);
-  const int ctiles = cache_tiles(p, cache_len(p, b)), per = ctiles + p.tree_tiles;
-  const int64_t u0 = before + (int64_t)head * unit_span(p, ctiles);
-  const int g0 = group_of(p, total, u0), g1 = group_of(p, total, u0 + per - 1);
+  const int u0 = n.before + head * unit_span(p, n.ctiles), u1 = u0 + n.ctiles + p.tree_tiles;
+  const Cut cut(p, n.total);
+  const int g0 = cut.of(u0), g1 = cut.of(u1 - 1);
   if (g0 == g1) return;                                 // one run holds the unit: it is written already
   const int r = (h - head * per_head) * p.nodes + t, block = r / p.rows_per_block, at = r % p.rows_per_block;
   float top = -INFINITY, sum = 0.0f, acc[E] = {};
   for (int first = g0; first <= g1; first += 32) {
-    // a lane holds one run's maximum and sum; runs without tiles (fewer tiles than runs) hold nothing
+    // a lane holds one run's maximum and sum (every run from the first to the last holds tiles of the unit)
     const int g = first + lane;
     int64_t slot = 0;
     float2 ml = make_float2(-INFINITY, 0.0f);
     if (g <= g1) {
-      const int64_t s0 = group_start(p, total, g), s1 = group_start(p, total, g + 1);
-      if (s0 < s1) {
-        slot = (((int64_t)g * 2 + (s0 >= u0 ? 0 : 1)) * p.row_blocks + block) * p.rows_per_block + at;
-        ml = p.part_ml[slot];
-      }
+      slot = (((int64_t)g * 2 + (cut.start(g) >= u0 ? 0 : 1)) * p.row_blocks + block) * p.rows_per_block + at;
+      ml = p.part_ml[slot];
     }
     float m = ml.x;
 #pragma unroll
@@ -215,13 +208,13 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
     sum *= fade;
 #pragma unroll
     for (int c = 0; c < E; ++c) acc[c] *= fade;
-    const int n = min(32, g1 - first + 1);
-    for (int i = 0; i < n; i += 4) {                    // four runs' loads in flight
+    const int runs = min(32, g1 - first + 1);
+    for (int i = 0; i < runs; i += 4) {                    // four runs' loads in flight
       float part[4][E], wi[4], si[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         wi[k] = __shfl_sync(0xFFFFFFFFu, weight, (i + k) & 31);
-        si[k] = i + k < n ? __shfl_sync(0xFFFFFFFFu, ml.y, (i + k) & 31) : 0.0f;
+        si[k] = i + k < runs ? __shfl_sync(0xFFFFFFFFu, ml.y, (i + k) & 31) : 0.0f;
         const int64_t at_k = __shfl_sync(0xFFFFFFFFu, slot, (i + k) & 31);
         const float *src = p.part + at_k * D + lane * E;
 #pragma unroll
@@ -229,7 +222,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (si[k] == 0.0f) continue;                    // nothing seen there (or no tiles)
+        if (si[k] == 0.0f) continue;                    // nothing seen there
         sum = fmaf(wi[k], si[k], sum);
 #pragma unroll
         for (int c = 0; c < E; ++c) acc[c] = fmaf(wi[k], part[k][c], acc[c]);
@@ -252,7 +245,9 @@ template <int D> int launch_simt(const Params &p, cudaStream_t stream) {
 
 template <typename T, int D> int launch_combine(const Params &p, cudaStream_t stream) {
   const int64_t rows = (int64_t)p.batch * p.q_heads * p.nodes;
-  LRQK_CUDA_TRY(launch_dependent(tree_combine_kernel<T, D>, dim3((unsigned)ceil_div64(rows, 8)), dim3(256), 0, stream, 0, p));
+  // A plain launch: as a dependent one its CTAs sat beside the last products and the pair took 2 us longer.
+  tree_combine_kernel<T, D><<<(unsigned)ceil_div64(rows, 8), 256, 0, stream>>>(p);
+  LRQK_LAUNCH_CHECK();
   return LRQK_OK;
 }
 
@@ -282,6 +277,7 @@ int plan(const lrqk_tree_args *a, Params &p) {
     if (p.groups < 1) return LRQK_EUNSUPPORTED;
   }
   p.tree_tiles = (p.nodes + p.tile_keys - 1) / p.tile_keys;
+  if ((int64_t)p.batch * p.cache_heads * (ceil_div64(p.capacity, p.tile_keys) + p.tree_tiles + p.unit_cost) >= 1 << 30) return LRQK_EUNSUPPORTED;
   return LRQK_OK;
 }
 

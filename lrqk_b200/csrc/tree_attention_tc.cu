@@ -52,8 +52,7 @@ struct Barriers {
   uint64_t decided[2][2][4], pair[2][4];    // [row block][half][32 rows]: the maximum in use is set; [row block][32 rows]
   float top[2][kBlockRows], sum[2][2][kBlockRows];
   uint32_t tmem, give_up, odd[2][4];        // odd: drafted rows of V with values out of range, 128 bits for each drafted tile
-  int64_t x0, x1, base;
-  int32_t seq;
+  int32_t x0, x1, base, seq;
 };
 
 // Bounded wait for a phase, suspended for up to 20 us a look: spinning on plain looks, the product warp alone issued 900
@@ -267,11 +266,9 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
   }
   pdl_wait();
   if (warp == 0) {
-    int64_t before, total;
-    count_tiles(p, 0, before, total);
-    const int64_t x0 = group_start(p, total, group), x1 = group_start(p, total, group + 1);
-    int seq = 0;
-    int64_t base = 0;
+    const Cut cut(p, count_tiles(p, 0).total);
+    const int x0 = cut.start(group), x1 = cut.start(group + 1);
+    int seq = 0, base = 0;
     if (x0 < x1) find_sequence(p, x0, seq, base);
     if (lane == 0) { bar.x0 = x0; bar.x1 = x1; bar.base = base; bar.seq = seq; }
   }

@@ -40,39 +40,47 @@ __device__ __forceinline__ int cache_len(const Params &p, int b) {
 __device__ __forceinline__ int cache_tiles(const Params &p, int len) { return (len + p.tile_keys - 1) / p.tile_keys; }
 __device__ __forceinline__ int unit_span(const Params &p, int ctiles) { return ctiles + p.tree_tiles + p.unit_cost; }
 
-// First tile of group g of `total` tiles; the group that holds tile x.
-__device__ __forceinline__ int64_t group_start(const Params &p, int64_t total, int g) { return total * g / p.groups; }
-__device__ __forceinline__ int group_of(const Params &p, int64_t total, int64_t x) { return (int)(((x + 1) * p.groups - 1) / total); }
+// The cut of `total` tiles (below 2^30, checked on the host) into runs: the first `more` runs have one tile more.
+struct Cut {
+  int each, more;
+  __device__ __forceinline__ Cut(const Params &p, int total) : each(total / p.groups), more(total - each * p.groups) {}
+  __device__ __forceinline__ int start(int g) const { return g * each + min(g, more); }
+  // the run that holds tile x (every tile is in one: with each = 0 only the first `more` runs hold any)
+  __device__ __forceinline__ int of(int x) const {
+    const int big = more * (each + 1);
+    return x < big ? x / (each + 1) : more + (x - big) / each;
+  }
+};
 
-// One warp: the tiles of all units of the sequences before `upto`, and of all sequences.
-__device__ __forceinline__ void count_tiles(const Params &p, int upto, int64_t &before, int64_t &total) {
+// One warp: the tiles of all sequences, of those before sequence `upto`, and of sequence `upto` itself (its own cache tiles).
+struct Count { int total, before, ctiles; };
+__device__ __forceinline__ Count count_tiles(const Params &p, int upto) {
   const int lane = threadIdx.x & 31;
-  int64_t s = 0, t = 0;
+  int s = 0, t = 0, own = 0;
   for (int b = lane; b < p.batch; b += 32) {
-    const int64_t n = (int64_t)p.cache_heads * unit_span(p, cache_tiles(p, cache_len(p, b)));
+    const int c = cache_tiles(p, cache_len(p, b)), n = p.cache_heads * unit_span(p, c);
     t += n;
     if (b < upto) s += n;
+    if (b == upto) own = c;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
-  }
-  before = s;
-  total = t;
+  Count r;
+  r.total = __reduce_add_sync(0xFFFFFFFFu, t);
+  r.before = __reduce_add_sync(0xFFFFFFFFu, s);
+  r.ctiles = __reduce_add_sync(0xFFFFFFFFu, own);
+  return r;
 }
 
 // One warp: the sequence that tile x belongs to and the first tile of that sequence.
-__device__ __forceinline__ void find_sequence(const Params &p, int64_t x, int &seq, int64_t &base) {
+__device__ __forceinline__ void find_sequence(const Params &p, int x, int &seq, int &base) {
   const int lane = threadIdx.x & 31;
-  int64_t run = 0;
+  int run = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     const int b = b0 + lane;
-    const int64_t n = b < p.batch ? (int64_t)p.cache_heads * unit_span(p, cache_tiles(p, cache_len(p, b))) : 0;
-    int64_t sum = n;
+    const int n = b < p.batch ? p.cache_heads * unit_span(p, cache_tiles(p, cache_len(p, b))) : 0;
+    int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+      const int up = __shfl_up_sync(0xFFFFFFFFu, sum, o);
       if (lane >= o) sum += up;
     }
     const unsigned hit = __ballot_sync(0xFFFFFFFFu, b < p.batch && run + sum > x);
@@ -90,18 +98,18 @@ __device__ __forceinline__ void find_sequence(const Params &p, int64_t x, int &s
 
 // The segments of one group's run [x0, x1): for (Walk w(...); w.valid(); w.next(p)).
 struct Walk {
-  int64_t x0, end, base, unit;   // the run; first tile of the sequence, of the unit
+  int x0, end, base, unit;       // the run; first tile of the sequence, of the unit
   int b, len, ctiles, per;       // sequence, its length, cache tiles and own tiles of a unit
   int head, t0, t1;              // the segment: cache head, tiles [t0, t1) of the unit
-  __device__ __forceinline__ Walk(const Params &p, int64_t run0, int64_t run1, int seq, int64_t seq_base)
+  __device__ __forceinline__ Walk(const Params &p, int run0, int run1, int seq, int seq_base)
       : x0(run0), end(run1), base(seq_base), b(seq) {
     if (x0 >= end) { unit = end; return; }
     size(p);
     const int span = unit_span(p, ctiles);
-    head = (int)((x0 - base) / span);
-    unit = base + (int64_t)head * span;
-    t0 = (int)(x0 - unit);
-    t1 = (int)min((int64_t)per, end - unit);
+    head = (x0 - base) / span;
+    unit = base + head * span;
+    t0 = x0 - unit;
+    t1 = min(per, end - unit);
     if (t0 >= per) next(p);      // the run starts on empty tiles
   }
   __device__ __forceinline__ void size(const Params &p) {
@@ -121,7 +129,7 @@ struct Walk {
       size(p);
     }
     t0 = 0;
-    t1 = (int)min((int64_t)per, end - unit);
+    t1 = min(per, end - unit);
   }
   // where the partial of this segment goes: to slot 0 for the unit that the run starts in, to slot 1 for the one it ends in
   __device__ __forceinline__ int64_t slot(const Params &p, int group, int block) const {
