@@ -6,18 +6,21 @@
 //
 // Every one of these decisions is a comparison of sums, and a sum in fp32 decides differently from one in another order as
 // soon as a number falls near a border.  So weights are 45-bit whole numbers, W = round(2^44 w), from an exponential in
-// double (own: Taylor to the fifth order around 64 table values of 2^x, Tang's table method): whole-number sums have no
+// double (own: Taylor to the fourth order around 128 table values of 2^x, Tang's table method): whole-number sums have no
 // order, are the same for any cluster size, and agree with 64-bit floating sums to 2^-34 of the mass.
 //
 // A row's logits are read once, into the shared memory of the cluster's CTAs (1, 2, 4 or 8: enough SMs for few rows,
-// enough memory for large vocabularies).  Top-k and top-p look for the key (an order-preserving integer of a logit) at
-// which a running count or mass crosses its target: histograms of counts or of the weights' three 15-bit limbs (the
-// sums of 2^17 of them fit 32 bits, so shared-memory atomics stay 32-bit), merged over the cluster in distributed shared
-// memory; the first level bins by distance from the maximum, which spreads the crowded exponents, the next ones by key
-// until one key is left.  Positions in index order (ties at a border, the final choice) come from per-warp sums of
-// contiguous chunks and a second look at one chunk.
+// enough memory for large vocabularies).  Top-k and top-p look for the place in the descending order where a running count
+// or mass crosses its target: a histogram of counts, or of the weights' three 15-bit limbs (the sums of 2^17 of them fit
+// 32 bits, so shared-memory atomics stay 32-bit), over bins of distance from the maximum, merged over the cluster in
+// distributed shared memory, finds the bin; its tokens, a few hundred at most, go to a list that every CTA gets and
+// settles by itself, ties included.  A bin with more (equal logits by the thousand) is cut further by key, an
+// order-preserving integer of a logit, and ties are counted in index order.  Where top-k leaves a few hundred tokens in
+// all, the list takes them all and the first CTA does the rest.  The final choice, in index order, comes from per-warp
+// sums of contiguous chunks and a second look at one chunk.
 //
-// Bound: latency of the cluster barriers for few rows; fp64 and shared-memory atomics for many.
+// Bound: the latency of the cluster barriers for few rows (each merge is two of them, 2.7 us with the reads between);
+// instructions -- the double exponential, three atomics a token -- for many.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -27,8 +30,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kSampThreads = 1024, kSampWarps = 32, kSampBins = 512, kSampMaxCluster = 8;
+constexpr int kSampThreads = 512, kSampWarps = 16, kSampBins = 512, kSampMaxCluster = 8;
 constexpr int kFracBits = 44;                          // of a weight
+constexpr int kTable = 128;                            // values of 2^(j / 128)
+constexpr int kList = 512;                             // tokens of a list (a CTA may add kList / cluster size)
 constexpr size_t kSampSliceBytes = 208 * 1024;         // logits of one CTA
 
 struct SampleParams {
@@ -44,9 +49,14 @@ struct SampleParams {
 };
 
 struct SampleShared {
-  double table[64];
-  unsigned long long merged[kSampBins], best[kSampMaxCluster], xsum[2][kSampMaxCluster], wsum[kSampWarps], pick_above, pick_in, pick_total;
-  uint32_t hist[3][kSampBins], low[kSampMaxCluster], wlow[kSampWarps], tie_index, pick_bin;
+  double table[kTable];
+  unsigned long long merged[kSampBins], xsum[2][kSampMaxCluster], wsum[kSampWarps], total[2], pick_above, pick_in, pick_total;
+  union {
+    uint32_t hist[3][kSampBins];
+    struct { unsigned long long entry[kList], weight[kList]; } list;   // key and inverted index; its weight (0: dropped)
+  };
+  float high[kSampMaxCluster], low[kSampMaxCluster], whigh[kSampWarps], wlow[kSampWarps];
+  uint32_t count[kSampMaxCluster], mine, tie_index, pick_bin, index;
 };
 
 template <typename T> struct SampKey;                  // order-preserving keys and back
@@ -61,6 +71,14 @@ template <> struct SampKey<__nv_bfloat16> {
   __device__ static __forceinline__ float value(uint32_t k) { return __uint_as_float((k & 0x8000u) ? (k ^ 0x8000u) << 16 : ~k << 16); }
 };
 
+__device__ __forceinline__ void pack(float *to, const float (&f)[4]) { *reinterpret_cast<float4 *>(to) = make_float4(f[0], f[1], f[2], f[3]); }
+__device__ __forceinline__ void pack(__nv_bfloat16 *to, const float (&f)[8]) {   // (the values are bf16: an exact repacking)
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = (__float_as_uint(f[2 * i]) >> 16) | (__float_as_uint(f[2 * i + 1]) & 0xFFFF0000u);
+  *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 struct Cut { uint32_t key, index; };                   // kept: larger keys, and this key up to this index
 
 template <typename T> struct Sampler {
@@ -70,8 +88,8 @@ template <typename T> struct Sampler {
   T *vals;
   cg::cluster_group cluster;
   int rank, csize, warp, lane, flip;
-  float top;                                           // the row's maximum
-  double top_d, c64;                                   // 64 log2(e) / T
+  float top, dust;                                     // the row's maximum; logits up to here weigh nothing
+  double per_log;                                      // 128 log2(e) / T
 
   __device__ Sampler(const SampleParams &params, SampleShared &shared, T *values)
       : p(params), sm(shared), vals(values), cluster(cg::this_cluster()), rank((int)cluster.block_rank()),
@@ -97,15 +115,16 @@ template <typename T> struct Sampler {
   // round(2^44 exp((f - top) / T)), f <= top
   __device__ __forceinline__ unsigned long long weight(float f) const {
     if (f == top) return 1ull << kFracBits;
-    const double y = ((double)f - top_d) * c64;        // 64ths of an octave
-    if (!(y > -64.0 * (kFracBits + 1))) return 0ull;
-    const double magic = 6755399441055744.0;           // 1.5 * 2^52: the sum's low bits are the nearest whole number
+    if (!(f > dust)) return 0ull;
+    const double y = ((double)f - (double)top) * per_log; // 128ths of an octave, above -6100
+    const double magic = 6755399441055744.0;              // 1.5 * 2^52: the sum's low bits are the nearest whole number
     const double n = y + magic;
-    const int k = (int)(unsigned)__double_as_longlong(n);
-    const double z = (y - (n - magic)) * 0.010830424696249145;   // ln(2) / 64; |z| < 0.0055, next term of the series below 2^-54
-    const double e = fma(z, fma(z, fma(z, fma(z, fma(z, 1.0 / 120.0, 1.0 / 24.0), 1.0 / 6.0), 0.5), 1.0), 1.0) * sm.table[k & 63];
-    const double scaled = __longlong_as_double(__double_as_longlong(e) + ((long long)((k >> 6) + kFracBits) << 52));
-    return (unsigned long long)(__double_as_longlong(scaled + 4503599627370496.0) - __double_as_longlong(4503599627370496.0));
+    const int k = __double2loint(n);
+    const double r = y - (n - magic);                     // |r ln(2) / 128| < 0.0028: the series' next term is below 2^-49
+    const double e = fma(r, fma(r, fma(r, fma(r, 3.583032305400251e-11, 2.6466421444330967e-08), 1.4662262387640423e-05), 0.0054152123481245725), 1.0) * sm.table[k & (kTable - 1)];
+    const double scaled = __hiloint2double(__double2hiint(e) + (((k >> 7) + kFracBits) << 20), __double2loint(e));
+    const double whole = scaled + 4503599627370496.0;     // 2^52
+    return ((unsigned long long)(uint32_t)(__double2hiint(whole) - 0x43300000) << 32) | (uint32_t)__double2loint(whole);
   }
 
   __device__ __forceinline__ bool inside(const Cut &c, float f, int at) const {
@@ -113,24 +132,28 @@ template <typename T> struct Sampler {
     return k > c.key || (k == c.key && index_of(at) <= c.index);
   }
 
-  // Merge the histograms of the cluster and find the bin in which the running sum from bin 0 reaches `target`
-  // (target 0: `target_of` makes it from the total).  MASS: three limbs; else counts in hist[0].
+  __device__ __forceinline__ unsigned long long entry(float f, int at) const {
+    return ((unsigned long long)SampKey<T>::of(f) << 32) | (0xFFFFFFFFu - index_of(at));   // descending: larger key, lower index
+  }
+
+  // Merge the histograms of the cluster and find the bin in which the running sum from bin 0 reaches target_of(total).
+  // MASS: three limbs; else counts in hist[0].
   template <bool MASS, typename F> __device__ void pick(F target_of) {
     cluster.sync();
-    for (int i = threadIdx.x; i < kSampBins / csize; i += kSampThreads) {
-      const int bin = rank * (kSampBins / csize) + i;
-      unsigned long long s = 0;
-      for (int c = 0; c < csize; ++c) {
-        const uint32_t *h = cluster.map_shared_rank(&sm.hist[0][0], c);
-        s += h[bin];
-        if (MASS) s += ((unsigned long long)h[kSampBins + bin] << 15) + ((unsigned long long)h[2 * kSampBins + bin] << 30);
-      }
-      for (int c = 0; c < csize; ++c) cluster.map_shared_rank(sm.merged, c)[bin] = s;
+    {
+      // a thread per bin of this CTA's share and source; the sources of a bin are neighbouring lanes
+      const int bin = rank * (kSampBins / csize) + threadIdx.x / csize, from = threadIdx.x % csize;
+      const uint32_t *h = cluster.map_shared_rank(&sm.hist[0][0], from);
+      unsigned long long v = h[bin];
+      if (MASS) v += ((unsigned long long)h[kSampBins + bin] << 15) + ((unsigned long long)h[2 * kSampBins + bin] << 30);
+      for (int o = 1; o < csize; o <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+      cluster.map_shared_rank(sm.merged, from)[bin] = v;
     }
     cluster.sync();
     if (warp == 0) {
       constexpr int PER = kSampBins / 32;
       unsigned long long mine = 0;
+#pragma unroll
       for (int i = 0; i < PER; ++i) mine += sm.merged[lane * PER + i];
       unsigned long long sum = mine;
 #pragma unroll
@@ -166,15 +189,54 @@ template <typename T> struct Sampler {
   }
 
   __device__ __forceinline__ void clear() {
+    __syncthreads();
     for (int i = threadIdx.x; i < 3 * kSampBins; i += kSampThreads) (&sm.hist[0][0])[i] = 0u;
     __syncthreads();
   }
 
+  // The tokens that `wanted` names, of all CTAs, into every CTA's list (in the histograms' place); their number, or -1 if
+  // one CTA has more than its share of the list holds.
+  template <typename F> __device__ int gather(F wanted) {
+    const uint32_t share = kList / csize;
+    if (threadIdx.x == 0) sm.mine = 0u;                // (the list itself is not cleared: peers may be filling it already)
+    __syncthreads();
+    each([&](float f, int at) {
+      if (!wanted(f, at)) return;
+      const uint32_t to = atomicAdd(&sm.mine, 1u);
+      if (to < share) {
+        const unsigned long long e = entry(f, at);
+        for (int c = 0; c < csize; ++c) cluster.map_shared_rank(sm.list.entry, c)[rank * share + to] = e;
+      }
+    });
+    __syncthreads();
+    if (threadIdx.x < (unsigned)csize) cluster.map_shared_rank(sm.count, threadIdx.x)[rank] = sm.mine;
+    cluster.sync();
+    // closed up: thread i takes entry i of all
+    int n = 0, from = -1;
+    bool fits = true;
+    for (int c = 0; c < csize; ++c) {
+      const int m = (int)sm.count[c];
+      fits = fits && m <= (int)share;
+      if (from < 0 && (int)threadIdx.x < n + m) from = c * (int)share + (int)threadIdx.x - n;
+      n += m;
+    }
+    if (!fits) {
+      cluster.sync();                                  // everyone has read the counts
+      return -1;
+    }
+    const unsigned long long e = from >= 0 ? sm.list.entry[from] : 0ull;
+    __syncthreads();
+    if (from >= 0) sm.list.entry[threadIdx.x] = e;
+    return n;
+  }
+
+  __device__ __forceinline__ float value_of(unsigned long long e) const { return SampKey<T>::value((uint32_t)(e >> 32)); }
+
   // Cut the tokens inside `cut` to those from the largest down to where the count (MASS: the mass) reaches its target.
-  // lowest: key of the smallest candidate.
-  template <bool MASS> __device__ void narrow(Cut &cut, uint32_t lowest, unsigned long long count, double share) {
-    uint32_t khi = SampKey<T>::of(top), klo = max(lowest, cut.key);
-    unsigned long long target = count, above = 0, in = 0;
+  // lowest: the smallest candidate.  Returns -1; or, for a count whose tokens all fit the list, their number, and makes no cut.
+  template <bool MASS> __device__ int narrow(Cut &cut, float lowest, unsigned long long count, double share) {
+    uint32_t khi = SampKey<T>::of(top), klo = max(SampKey<T>::of(lowest), cut.key);
+    unsigned long long target, above, in;
     // level 0: bins by distance from the maximum.  (Halved, so that the range of any two floats is finite.)
     const float half_top = 0.5f * top, range = half_top - 0.5f * SampKey<T>::value(klo);
     const float per = (float)kSampBins / range;
@@ -187,7 +249,7 @@ template <typename T> struct Sampler {
       }
     });
     const auto first_target = [&](unsigned long long total) {
-      if (!MASS) return min(count, total);               // fewer candidates than asked for: all of them
+      if (!MASS) return min(count, total);             // fewer candidates than asked for: all of them
       const double t = ceil(share * (double)total);    // before < share * total, for whole numbers before
       return t < 1.0 ? 1ull : min(total, (unsigned long long)t);
     };
@@ -196,6 +258,11 @@ template <typename T> struct Sampler {
     above = sm.pick_above;
     in = sm.pick_in;
     target = first_target(sm.pick_total);
+    if (!MASS && above + in <= kList / 2) {
+      const int n = gather([&](float f, int at) { return candidate(f) && bin0(f) <= b0; });
+      if (n >= 0) return n;
+    }
+    const Cut old = cut;
     if (khi != klo) {
       // keys that can lie in that bin (a little wider: the test itself is bin0)
       const float slack = (fabsf(top) + 2.0f * range) * 0x1p-20f + 1e-37f, step = 2.0f * range / kSampBins;
@@ -203,38 +270,110 @@ template <typename T> struct Sampler {
       if (b0 < kSampBins - 1) klo = max(klo, SampKey<T>::of(top - step * (float)(b0 + 1) - slack));
       if (klo > khi) klo = khi;
     }
-    while (khi != klo) {
+    const auto in_reach = [&](float f, int at) {
+      if (!candidate(f) || bin0(f) != b0) return false;
+      const uint32_t k = SampKey<T>::of(f);
+      return k <= khi && k >= klo && inside(old, f, at);
+    };
+    for (;;) {
+      // at most so many tokens are in reach: all, if each weighs no less than the smallest key
+      const unsigned long long least = MASS ? weight(SampKey<T>::value(klo)) : 1ull;
+      if (least && in / least <= kList / 2) {
+        const int n = gather(in_reach);
+        if (n >= 0) {
+          settle<MASS>(cut, n, target - above);
+          return -1;
+        }
+      }
+      if (khi == klo) break;
       const int shift = max(0, 32 - __clz((int)(khi - klo)) - 9);        // 512 bins of 2^shift keys
       clear();
       each([&](float f, int at) {
-        if (!candidate(f) || bin0(f) != b0) return;
-        const uint32_t k = SampKey<T>::of(f);
-        if (k > khi || k < klo || !inside(cut, f, at)) return;
+        if (!in_reach(f, at)) return;
         const unsigned long long w = MASS ? weight(f) : 1ull;
-        if (w) add<MASS>((khi - k) >> shift, w);
+        if (w) add<MASS>((khi - SampKey<T>::of(f)) >> shift, w);
       });
       pick<MASS>([&](unsigned long long) { return target - above; });
       above += sm.pick_above;
       in = sm.pick_in;
       khi -= sm.pick_bin << shift;
-      klo = shift == 0 || khi - klo < (1u << shift) ? (shift == 0 ? khi : klo) : khi - (1u << shift) + 1u;
-      __syncthreads();
+      klo = shift == 0 ? khi : khi - klo < (1u << shift) ? klo : khi - (1u << shift) + 1u;
     }
+    // equal logits by the hundred: the need-th of them, in index order
     const unsigned long long each_w = MASS ? weight(SampKey<T>::value(khi)) : 1ull;
     const unsigned long long ties = each_w ? in / each_w : 0ull, need = each_w ? (target - above + each_w - 1) / each_w : 1ull;
-    Cut got{khi, khi == cut.key ? cut.index : 0xFFFFFFFFu};
+    cut.index = khi == old.key ? old.index : 0xFFFFFFFFu;
+    cut.key = khi;
     if (need < ties) {
-      // the need-th of the equal keys, in index order
-      const Cut old = cut;
       locate([&](float f, int at) -> unsigned long long { return SampKey<T>::of(f) == khi && candidate(f) && inside(old, f, at) ? 1ull : 0ull; },
              [&](unsigned long long) { return need - 1; },
              [&](uint32_t index, float, unsigned long long) {
                for (int c = 0; c < csize; ++c) *cluster.map_shared_rank(&sm.tie_index, c) = index;
              });
       cluster.sync();
-      got.index = sm.tie_index;
+      cut.index = sm.tie_index;
     }
-    cut = got;
+    return -1;
+  }
+
+  // The list's n tokens settle the cut: the one at which their count (MASS: mass), in descending order, reaches `target`.
+  template <bool MASS> __device__ void settle(Cut &cut, int n, unsigned long long target) {
+    const int i = threadIdx.x;
+    const unsigned long long e = i < n ? sm.list.entry[i] : 0ull, w = i < n ? (MASS ? weight(value_of(e)) : 1ull) : 0ull;
+    if (MASS && i < n) sm.list.weight[i] = w;
+    __syncthreads();
+    if (i < n) {
+      unsigned long long before = 0;
+      for (int j = 0; j < n; ++j)
+        if (sm.list.entry[j] > e) before += MASS ? sm.list.weight[j] : 1ull;
+      if (before < target && before + w >= target) { sm.pick_above = e; }
+    }
+    __syncthreads();
+    cut.key = (uint32_t)(sm.pick_above >> 32);
+    cut.index = 0xFFFFFFFFu - (uint32_t)sm.pick_above;
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ unsigned long long block_sum(unsigned long long v, int slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    if (lane == 0) sm.wsum[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+      unsigned long long t = lane < kSampWarps ? sm.wsum[lane] : 0ull;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+      if (lane == 0) sm.total[slot] = t;
+    }
+    __syncthreads();
+    return sm.total[slot];
+  }
+
+  // Few tokens are left and the list holds them all (n): top-k, top-p, min-p and the choice, in one CTA.
+  template <typename G, typename F> __device__ void finish(int n, unsigned long long k, double share, bool nucleus, unsigned long long floor_w, G target_of, F found) {
+    const int i = threadIdx.x;
+    const unsigned long long e = i < n ? sm.list.entry[i] : 0ull, w = i < n ? weight(value_of(e)) : 0ull;
+    if (i < n) sm.list.weight[i] = w;
+    __syncthreads();
+    unsigned long long before = 0;                     // mass of the larger ones
+    uint32_t rank_of = 0;
+    if (i < n)
+      for (int j = 0; j < n; ++j)
+        if (sm.list.entry[j] > e) { before += sm.list.weight[j]; ++rank_of; }
+    const bool in_k = i < n && rank_of < k;
+    const unsigned long long total = block_sum(in_k ? w : 0ull, 0);
+    const double t = ceil(share * (double)total);
+    const unsigned long long target = t < 1.0 ? 1ull : min(total, (unsigned long long)t);
+    const unsigned long long kept = in_k && (!nucleus || before < target) && w >= floor_w ? w : 0ull;
+    __syncthreads();
+    if (i < n) sm.list.weight[i] = kept;
+    const unsigned long long sum = block_sum(kept, 1), chosen = target_of(sum);
+    if (kept) {
+      unsigned long long mass = 0;                     // of the kept ones of lower index (larger inverted index)
+      for (int j = 0; j < n; ++j)
+        if ((uint32_t)sm.list.entry[j] > (uint32_t)e) mass += sm.list.weight[j];
+      if (mass <= chosen && mass + kept > chosen) found(0xFFFFFFFFu - (uint32_t)e, value_of(e), sum);
+    }
   }
 
   // The first token, in index order, at which the cumulative weight exceeds target_of(total): found(index, value, total)
@@ -304,20 +443,17 @@ __global__ void __launch_bounds__(kSampThreads, 1) sample_kernel(const __grid_co
   Sampler<T> s(p, sm, reinterpret_cast<T *>(smem_raw));
   const int row = blockIdx.x / s.csize;
   constexpr int VE = Sampler<T>::VE, STEP = Sampler<T>::STEP;
-  if (threadIdx.x < 64) sm.table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 64.0));
+  if (threadIdx.x < kTable) sm.table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / kTable));
   pdl_wait();
 
   // ---- the row's slice into shared memory; NaN counts as -inf, and so does what lies behind the vocabulary -----------
   const T *src = static_cast<const T *>(p.logits) + (int64_t)row * p.row_stride;
   const int base = s.warp * p.chunk;
-  unsigned long long best = 0;
-  uint32_t low = SampKey<T>::kTop;
-  const auto note = [&](float f, uint32_t index) {
-    if (f > -INFINITY) {
-      const uint32_t k = SampKey<T>::of(f);
-      best = max(best, ((unsigned long long)k << 32) | (0xFFFFFFFFu - index));
-      low = min(low, k);
-    }
+  float high = -INFINITY, low = INFINITY;              // of the logits above -inf
+  const auto note = [&](float &f) {
+    f = fmaxf(f, -INFINITY);                           // (fmaxf drops a NaN)
+    high = fmaxf(high, f);
+    low = fminf(low, f > -INFINITY ? f : INFINITY);
   };
   if (p.vectors) {
 #pragma unroll 4
@@ -332,11 +468,8 @@ __global__ void __launch_bounds__(kSampThreads, 1) sample_kernel(const __grid_co
         for (int j = 0; j < VE; ++j) f[j] = index + j < (uint32_t)p.vocab ? Elt<T>::to_float(src[index + j]) : -INFINITY;
       }
 #pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        if (f[j] != f[j]) f[j] = -INFINITY;
-        s.vals[at + j] = Elt<T>::from_float(f[j]);
-        note(f[j], index + j);
-      }
+      for (int j = 0; j < VE; ++j) note(f[j]);
+      pack(s.vals + at, f);
     }
   } else {
 #pragma unroll 4
@@ -344,71 +477,82 @@ __global__ void __launch_bounds__(kSampThreads, 1) sample_kernel(const __grid_co
       const int at = base + i + s.lane;
       const uint32_t index = s.index_of(at);
       float f = index < (uint32_t)p.vocab ? Elt<T>::to_float(src[index]) : -INFINITY;
-      if (f != f) f = -INFINITY;
+      note(f);
       s.vals[at] = Elt<T>::from_float(f);
-      note(f, index);
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    best = max(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
-    low = min(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
+    high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, o));
+    low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
   }
-  if (s.lane == 0) { sm.wsum[s.warp] = best; sm.wlow[s.warp] = low; }
+  if (s.lane == 0) { sm.whigh[s.warp] = high; sm.wlow[s.warp] = low; }
+  if (threadIdx.x == 0) sm.index = 0xFFFFFFFFu;
   s.cluster.sync();                                    // every CTA of the cluster runs: its shared memory can be written
-  best = sm.wsum[s.lane];
-  low = sm.wlow[s.lane];
+  if (s.warp == 0) {
+    high = sm.whigh[s.lane & (kSampWarps - 1)];
+    low = sm.wlow[s.lane & (kSampWarps - 1)];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    best = max(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
-    low = min(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
-  }
-  if (threadIdx.x < (unsigned)s.csize) {
-    *s.cluster.map_shared_rank(&sm.best[s.rank], threadIdx.x) = best;
-    *s.cluster.map_shared_rank(&sm.low[s.rank], threadIdx.x) = low;
+    for (int o = 8; o > 0; o >>= 1) {
+      high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, o));
+      low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
+    }
+    if (s.lane < s.csize) {
+      *s.cluster.map_shared_rank(&sm.high[s.rank], s.lane) = high;
+      *s.cluster.map_shared_rank(&sm.low[s.rank], s.lane) = low;
+    }
   }
   s.cluster.sync();
-  for (int c = 0; c < s.csize; ++c) { best = max(best, sm.best[c]); low = min(low, sm.low[c]); }
+  high = sm.high[0];
+  low = sm.low[0];
+  for (int c = 1; c < s.csize; ++c) { high = fmaxf(high, sm.high[c]); low = fminf(low, sm.low[c]); }
+  s.top = high;
 
   const float t = p.temperature ? p.temperature[row] : p.temperature1;
   const bool first = s.rank == 0 && threadIdx.x == 0;
-  if (best == 0) {                                     // nothing but -inf and NaN: no token
+  if (high == -INFINITY) {                             // nothing but -inf and NaN: no token
     if (first) { p.tokens[row] = -1; if (p.logprobs) p.logprobs[row] = NAN; }
-  } else if (!(t > 0.0f)) {
-    if (first) { p.tokens[row] = 0xFFFFFFFFu - (uint32_t)best; if (p.logprobs) p.logprobs[row] = 0.0f; }
+  } else if (!(t > 0.0f)) {                            // the first maximum
+    s.each([&](float f, int at) { if (f == high) atomicMin(s.cluster.map_shared_rank(&sm.index, 0), s.index_of(at)); });
+    s.cluster.sync();
+    if (first) { p.tokens[row] = sm.index; if (p.logprobs) p.logprobs[row] = 0.0f; }
   } else {
-    s.top = SampKey<T>::value((uint32_t)(best >> 32));
-    s.top_d = (double)s.top;
-    s.c64 = 92.33248261893193 / (double)t;             // 64 log2(e) / T
-    if (s.top == INFINITY) low = (uint32_t)(best >> 32);
+    s.per_log = 184.6649652337873 / (double)t;         // 128 log2(e) / T
+    s.dust = __fsub_rd(high, 33.0f * t);               // 33 T below the maximum a weight rounds to nothing (2^-47)
+    if (high == INFINITY) low = high;
     const int k = p.top_k ? p.top_k[row] : p.top_k1;
     const float q = p.top_p ? p.top_p[row] : p.top_p1, m = p.min_p ? p.min_p[row] : p.min_p1, u = p.u[row];
-    Cut cut{0u, 0xFFFFFFFFu};
-    if (k > 0 && k < p.vocab) s.template narrow<false>(cut, low, (unsigned long long)k, 0.0);
-    if (q < 1.0f) s.template narrow<true>(cut, low, 0ull, (double)q);
     const unsigned long long floor_w = m > 0.0f ? (unsigned long long)__double2ull_rn(fmin((double)m, 1.0) * 17592186044416.0) : 0ull;
-    s.locate(
-        [&](float f, int at) -> unsigned long long {
-          if (!s.candidate(f) || !s.inside(cut, f, at)) return 0ull;
-          const unsigned long long w = s.weight(f);
-          return w >= floor_w ? w : 0ull;
-        },
-        [&](unsigned long long total) {
-          const double x = floor((double)u * (double)total);
-          return x > 0.0 ? min(total - 1, (unsigned long long)x) : 0ull;
-        },
-        [&](uint32_t index, float f, unsigned long long total) {
-          p.tokens[row] = index;
-          const double y = f == s.top ? 0.0 : ((double)f - s.top_d) / (double)t;
-          if (p.logprobs) p.logprobs[row] = (float)(y - log((double)total * 0x1p-44));
-        });
+    const auto target_of = [&](unsigned long long total) {
+      const double x = floor((double)u * (double)total);
+      return x > 0.0 ? min(total - 1, (unsigned long long)x) : 0ull;
+    };
+    const auto found = [&](uint32_t index, float f, unsigned long long total) {
+      p.tokens[row] = index;
+      const double y = f == high ? 0.0 : ((double)f - (double)high) / (double)t;
+      if (p.logprobs) p.logprobs[row] = (float)(y - log((double)total * 0x1p-44));
+    };
+    Cut cut{0u, 0xFFFFFFFFu};
+    int n = -1;
+    if (k > 0 && k < p.vocab) n = s.template narrow<false>(cut, low, (unsigned long long)k, 0.0);
+    if (n >= 0) {
+      if (s.rank == 0) s.finish(n, (unsigned long long)k, (double)q, q < 1.0f, floor_w, target_of, found);
+    } else {
+      if (q < 1.0f) s.template narrow<true>(cut, low, 0ull, (double)q);
+      s.locate(
+          [&](float f, int at) -> unsigned long long {
+            if (!s.candidate(f) || !s.inside(cut, f, at)) return 0ull;
+            const unsigned long long w = s.weight(f);
+            return w >= floor_w ? w : 0ull;
+          },
+          target_of, found);
+    }
   }
   s.cluster.sync();                                    // no CTA leaves while a peer may still write to it
 }
 
 template <typename T> int launch_sample(SampleParams &p, int rows, cudaStream_t stream) {
-  // Few rows: 8 CTAs each, for latency; more: fewer, as long as a slice fits.  (One row of 128256 bf16 logits, top-k 50 and
-  // top-p 0.9, by cluster size: see the note at the launch.)
+  // Few rows: 8 CTAs each, for latency; more: fewer, as long as a slice fits.
   constexpr int step = 32 * Elt<T>::kPerVec * kSampWarps;       // a slice is a whole number of these
   int csize = 1;
   const auto slice = [&](int c) { return ceil_div64(ceil_div64(p.vocab, c), step) * step; };
