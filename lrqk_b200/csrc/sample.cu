@@ -97,6 +97,11 @@ template <typename T> struct Sampler {
 
   __device__ __forceinline__ uint32_t index_of(int at) const { return (uint32_t)(rank * kSampWarps * p.chunk + at); }
 
+  // every value of this warp's chunk replaced
+  template <typename F> __device__ __forceinline__ void each_store(F fn) const {
+    for (int i = lane; i < p.chunk; i += 32) vals[warp * p.chunk + i] = Elt<T>::from_float(fn(Elt<T>::to_float(vals[warp * p.chunk + i])));
+  }
+
   // fn(value, place in the slice) for this warp's chunk, a lane's VE neighbours at a time
   template <typename F> __device__ __forceinline__ void each(F fn) const {
     const int base = warp * p.chunk;
@@ -109,12 +114,10 @@ template <typename T> struct Sampler {
     }
   }
 
-  // a logit that can carry mass: with a maximum of +inf only the infinite ones do
-  __device__ __forceinline__ bool candidate(float f) const { return f > -INFINITY && (top < INFINITY || f == top); }
+  __device__ __forceinline__ bool candidate(float f) const { return f > -INFINITY; }
 
   // round(2^44 exp((f - top) / T)), f <= top
   __device__ __forceinline__ unsigned long long weight(float f) const {
-    if (f == top) return 1ull << kFracBits;
     if (!(f > dust)) return 0ull;
     const double y = ((double)f - (double)top) * per_log; // 128ths of an octave, above -6100
     const double magic = 6755399441055744.0;              // 1.5 * 2^52: the sum's low bits are the nearest whole number
@@ -128,6 +131,7 @@ template <typename T> struct Sampler {
   }
 
   __device__ __forceinline__ bool inside(const Cut &c, float f, int at) const {
+    if (c.key == 0) return true;                       // (no cut yet)
     const uint32_t k = SampKey<T>::of(f);
     return k > c.key || (k == c.key && index_of(at) <= c.index);
   }
@@ -240,10 +244,10 @@ template <typename T> struct Sampler {
     // level 0: bins by distance from the maximum.  (Halved, so that the range of any two floats is finite.)
     const float half_top = 0.5f * top, range = half_top - 0.5f * SampKey<T>::value(klo);
     const float per = (float)kSampBins / range;
-    const auto bin0 = [&](float f) { return f == top ? 0 : min(kSampBins - 1, max(0, (int)((half_top - 0.5f * f) * per))); };
+    const auto bin0 = [&](float f) { return min(kSampBins - 1, max(0, (int)((half_top - 0.5f * f) * per))); };
     clear();
     each([&](float f, int at) {
-      if (candidate(f) && inside(cut, f, at)) {
+      if ((MASS ? f > dust : candidate(f)) && inside(cut, f, at)) {
         const unsigned long long w = MASS ? weight(f) : 1ull;
         if (w) add<MASS>(bin0(f), w);
       }
@@ -436,7 +440,7 @@ template <typename T> struct Sampler {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kSampThreads, 1) sample_kernel(const __grid_constant__ SampleParams p) {
+__global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_constant__ SampleParams p) {
   pdl_launch_dependents();
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ SampleShared sm;
@@ -519,7 +523,12 @@ __global__ void __launch_bounds__(kSampThreads, 1) sample_kernel(const __grid_co
   } else {
     s.per_log = 184.6649652337873 / (double)t;         // 128 log2(e) / T
     s.dust = __fsub_rd(high, 33.0f * t);               // 33 T below the maximum a weight rounds to nothing (2^-47)
-    if (high == INFINITY) low = high;
+    if (high == INFINITY) {                            // the infinite logits share the mass: as if they were 0, the rest nothing
+      s.each_store([](float f) { return f == INFINITY ? 0.0f : -INFINITY; });
+      __syncthreads();
+      s.top = high = low = 0.0f;
+      s.dust = -1.0f;
+    }
     const int k = p.top_k ? p.top_k[row] : p.top_k1;
     const float q = p.top_p ? p.top_p[row] : p.top_p1, m = p.min_p ? p.min_p[row] : p.min_p1, u = p.u[row];
     const unsigned long long floor_w = m > 0.0f ? (unsigned long long)__double2ull_rn(fmin((double)m, 1.0) * 17592186044416.0) : 0ull;
@@ -529,7 +538,7 @@ __global__ void __launch_bounds__(kSampThreads, 1) sample_kernel(const __grid_co
     };
     const auto found = [&](uint32_t index, float f, unsigned long long total) {
       p.tokens[row] = index;
-      const double y = f == high ? 0.0 : ((double)f - (double)high) / (double)t;
+      const double y = ((double)f - (double)high) / (double)t;
       if (p.logprobs) p.logprobs[row] = (float)(y - log((double)total * 0x1p-44));
     };
     Cut cut{0u, 0xFFFFFFFFu};
@@ -541,7 +550,7 @@ __global__ void __launch_bounds__(kSampThreads, 1) sample_kernel(const __grid_co
       if (q < 1.0f) s.template narrow<true>(cut, low, 0ull, (double)q);
       s.locate(
           [&](float f, int at) -> unsigned long long {
-            if (!s.candidate(f) || !s.inside(cut, f, at)) return 0ull;
+            if (!s.inside(cut, f, at)) return 0ull;
             const unsigned long long w = s.weight(f);
             return w >= floor_w ? w : 0ull;
           },
@@ -557,7 +566,7 @@ template <typename T> int launch_sample(SampleParams &p, int rows, cudaStream_t 
   int csize = 1;
   const auto slice = [&](int c) { return ceil_div64(ceil_div64(p.vocab, c), step) * step; };
   while (csize < kSampMaxCluster && (slice(csize) * (int64_t)sizeof(T) > (int64_t)kSampSliceBytes ||
-                                     (rows * csize * 2 <= kNumSMs && slice(csize) > step)))
+                                     (rows * csize <= kNumSMs && slice(csize) > step)))
     csize *= 2;
   if (slice(csize) * (int64_t)sizeof(T) > (int64_t)kSampSliceBytes) return LRQK_EUNSUPPORTED;
   p.chunk = (int)(slice(csize) / kSampWarps);

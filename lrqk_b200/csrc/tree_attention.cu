@@ -15,6 +15,14 @@ namespace {
 
 constexpr int kRows = 64, kKeys = 64, kThreads = 256;
 
+// Two fp32 multiply-adds in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)),
+      "l"(*reinterpret_cast<unsigned long long *>(&c)));
+  return *reinterpret_cast<float2 *>(&d);
+}
+
 template <int D> struct SimtShared {
   float q[kRows][D], k[kKeys][D + 4], v[kKeys][D], w[kRows][kKeys + 1];
 };
@@ -48,13 +56,14 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < VE; ++j) sm.q[r][c + j] = f[j];
     }
-    float top[4], sum[4], acc[4][4 * DC];
+    float top[4], sum[4];
+    float2 acc[4][2 * DC];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       top[i] = -INFINITY;
       sum[i] = 0.0f;
 #pragma unroll
-      for (int c = 0; c < 4 * DC; ++c) acc[i][c] = 0.0f;
+      for (int c = 0; c < 2 * DC; ++c) acc[i][c] = make_float2(0.0f, 0.0f);
     }
     const int tree_head = w.head / (p.cache_heads / p.tree_heads);
     for (int tile = w.t0; tile < w.t1; ++tile) {
@@ -79,7 +88,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
       }
       __syncthreads();
       if (works) {                                      // whole half-warps: a row's 16 threads stay together
-        float s[4][4] = {};
+        float2 s2[4][4] = {};                           // sums over even and odd columns
 #pragma unroll 4
         for (int c = 0; c < D; c += 4) {
           float4 a[4], b[4];
@@ -91,8 +100,14 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+              s2[i][j] = fma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y),
+                              fma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), s2[i][j]));
         }
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
         const unsigned half = (tid & 16) ? 0xFFFF0000u : 0x0000FFFFu;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -120,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
           for (int o = 8; o > 0; o >>= 1) add += __shfl_xor_sync(half, add, o);
           sum[i] = sum[i] * fade + add;
 #pragma unroll
-          for (int c = 0; c < 4 * DC; ++c) acc[i][c] *= fade;
+          for (int c = 0; c < 2 * DC; ++c) acc[i][c] = make_float2(acc[i][c].x * fade, acc[i][c].y * fade);
         }
         __syncwarp(half);
         for (int key = 0; key < n_keys; ++key) {
@@ -133,10 +148,8 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
             if (drafted && e == 0.0f) continue;         // a node that the row does not see adds nothing, whatever it holds
 #pragma unroll
             for (int c = 0; c < DC; ++c) {
-              acc[i][4 * c] = fmaf(e, v[c].x, acc[i][4 * c]);
-              acc[i][4 * c + 1] = fmaf(e, v[c].y, acc[i][4 * c + 1]);
-              acc[i][4 * c + 2] = fmaf(e, v[c].z, acc[i][4 * c + 2]);
-              acc[i][4 * c + 3] = fmaf(e, v[c].w, acc[i][4 * c + 3]);
+              acc[i][2 * c] = fma2(make_float2(e, e), make_float2(v[c].x, v[c].y), acc[i][2 * c]);
+              acc[i][2 * c + 1] = fma2(make_float2(e, e), make_float2(v[c].z, v[c].w), acc[i][2 * c + 1]);
             }
           }
         }
@@ -153,82 +166,110 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
         const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
         T *dst = static_cast<T *>(p.out) + at * D;
 #pragma unroll
-        for (int c = 0; c < 4 * DC; ++c) dst[tx * 4 + 64 * (c / 4) + c % 4] = Elt<T>::from_float(acc[i][c] * inv);
+        for (int c = 0; c < DC; ++c)
+          *reinterpret_cast<float4 *>(dst + tx * 4 + 64 * c) = make_float4(acc[i][2 * c].x * inv, acc[i][2 * c].y * inv, acc[i][2 * c + 1].x * inv, acc[i][2 * c + 1].y * inv);
         if (p.lse && tx == 0) p.lse[at] = sum[i] == 0.0f ? -INFINITY : (top[i] + log2f(sum[i])) * 0.6931471805599453f;
       } else {
         const int64_t at = w.slot(p, group, block) * p.rows_per_block + (r - row0);
 #pragma unroll
         for (int c = 0; c < DC; ++c)
-          *reinterpret_cast<float4 *>(p.part + at * D + tx * 4 + 64 * c) = make_float4(acc[i][4 * c], acc[i][4 * c + 1], acc[i][4 * c + 2], acc[i][4 * c + 3]);
+          *reinterpret_cast<float4 *>(p.part + at * D + tx * 4 + 64 * c) = make_float4(acc[i][2 * c].x, acc[i][2 * c].y, acc[i][2 * c + 1].x, acc[i][2 * c + 1].y);
         if (tx == 0) p.part_ml[at] = make_float2(top[i], sum[i]);
       }
     }
   }
 }
 
-// One warp per query row of a unit that was cut: the row's partials, folded in the order of the runs.
-template <typename T, int D>
+// One to eight warps (WARPS) per query row of a unit that was cut: each folds every WARPS-th of the row's partials, in the order
+// of the runs, the first folds theirs.
+template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Params p) {
   constexpr int E = D / 32;                             // columns of a lane
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);  // (batch * q_heads * nodes is below 2^31)
-  if (row >= p.batch * p.q_heads * p.nodes) return;
+  __shared__ float rows[8][D], row_top[8], row_sum[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WARPS;
+  const int row = blockIdx.x * (8 / WARPS) + warp / WARPS;   // (batch * q_heads * nodes is below 2^31)
+  const bool exists = row < p.batch * p.q_heads * p.nodes;
   const int t = row % p.nodes, h = row / p.nodes % p.q_heads, b = row / p.nodes / p.q_heads;
   const int32_t broken = p.status ? *reinterpret_cast<volatile int32_t *>(p.status) : 0;
   const Count n = count_tiles(p, b);
   T *dst = static_cast<T *>(p.out) + (int64_t)row * D + lane * E;
+  const int per_head = p.q_heads / p.cache_heads, head = h / per_head;
+  const int u0 = n.before + head * unit_span(p, n.ctiles), u1 = u0 + n.ctiles + p.tree_tiles;
+  const Cut cut(p, n.total);
+  const int g0 = exists ? cut.of(u0) : 0, g1 = exists ? cut.of(u1 - 1) : 0;
+  const bool folds = exists && !broken && g0 != g1;     // (a unit that one run holds is written already)
+  float top = -INFINITY, sum = 0.0f, acc[E] = {};
+  if (folds) {
+    const int r = (h - head * per_head) * p.nodes + t, block = r / p.rows_per_block, at = r % p.rows_per_block;
+    for (int first = g0 + part; first <= g1; first += 32 * WARPS) {
+      // a lane holds one run's maximum and sum (every run from the first to the last holds tiles of the unit)
+      const int g = first + lane * WARPS;
+      int64_t slot = 0;
+      float2 ml = make_float2(-INFINITY, 0.0f);
+      if (g <= g1) {
+        slot = (((int64_t)g * 2 + (cut.start(g) >= u0 ? 0 : 1)) * p.row_blocks + block) * p.rows_per_block + at;
+        ml = p.part_ml[slot];
+      }
+      float m = ml.x;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      m = fmaxf(m, top);
+      const float ref = m == -INFINITY ? 0.0f : m, fade = exp2f(top - ref), weight = exp2f(ml.x - ref);
+      top = m;
+      sum *= fade;
+#pragma unroll
+      for (int c = 0; c < E; ++c) acc[c] *= fade;
+      const int runs = min(32, (g1 - first) / WARPS + 1);
+      for (int i = 0; i < runs; i += 8) {               // eight runs' loads in flight
+        float got[8][E], wi[8], si[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          wi[k] = __shfl_sync(0xFFFFFFFFu, weight, (i + k) & 31);
+          si[k] = __shfl_sync(0xFFFFFFFFu, ml.y, (i + k) & 31);
+          const int64_t at_k = __shfl_sync(0xFFFFFFFFu, slot, (i + k) & 31);
+          if (i + k >= runs) si[k] = 0.0f;
+          const float *src = p.part + at_k * D + lane * E;
+#pragma unroll
+          for (int c = 0; c < E; ++c) got[k][c] = si[k] != 0.0f ? src[c] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (si[k] == 0.0f) continue;                  // nothing seen there
+          sum = fmaf(wi[k], si[k], sum);
+#pragma unroll
+          for (int c = 0; c < E; ++c) acc[c] = fmaf(wi[k], got[k][c], acc[c]);
+        }
+      }
+    }
+  }
+  if (WARPS > 1) {
+#pragma unroll
+    for (int c = 0; c < E; ++c) rows[warp][lane * E + c] = acc[c];
+    if (lane == 0) { row_top[warp] = top; row_sum[warp] = sum; }
+    __syncthreads();
+    if (part != 0) return;
+    float m = top;
+    for (int k = 1; k < WARPS; ++k) m = fmaxf(m, row_top[warp + k]);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < E; ++c) acc[c] = 0.0f;
+    for (int k = 0; k < WARPS; ++k) {
+      if (row_sum[warp + k] == 0.0f) continue;
+      const float wk = exp2f(row_top[warp + k] - ref);
+      sum = fmaf(wk, row_sum[warp + k], sum);
+#pragma unroll
+      for (int c = 0; c < E; ++c) acc[c] = fmaf(wk, rows[warp + k][lane * E + c], acc[c]);
+    }
+    top = m;
+  }
+  if (part != 0 || !exists) return;
   if (broken != 0) {                                    // a wait ran out: no row can be trusted
     for (int c = 0; c < E; ++c) dst[c] = Elt<T>::from_float(NAN);
     if (p.lse && lane == 0) p.lse[row] = NAN;
     return;
   }
-  const int per_head = p.q_heads / p.cache_heads, head = h / per_head;
-  const int u0 = n.before + head * unit_span(p, n.ctiles), u1 = u0 + n.ctiles + p.tree_tiles;
-  const Cut cut(p, n.total);
-  const int g0 = cut.of(u0), g1 = cut.of(u1 - 1);
-  if (g0 == g1) return;                                 // one run holds the unit: it is written already
-  const int r = (h - head * per_head) * p.nodes + t, block = r / p.rows_per_block, at = r % p.rows_per_block;
-  float top = -INFINITY, sum = 0.0f, acc[E] = {};
-  for (int first = g0; first <= g1; first += 32) {
-    // a lane holds one run's maximum and sum (every run from the first to the last holds tiles of the unit)
-    const int g = first + lane;
-    int64_t slot = 0;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (g <= g1) {
-      slot = (((int64_t)g * 2 + (cut.start(g) >= u0 ? 0 : 1)) * p.row_blocks + block) * p.rows_per_block + at;
-      ml = p.part_ml[slot];
-    }
-    float m = ml.x;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    m = fmaxf(m, top);
-    const float ref = m == -INFINITY ? 0.0f : m, fade = exp2f(top - ref);
-    const float weight = exp2f(ml.x - ref);
-    top = m;
-    sum *= fade;
-#pragma unroll
-    for (int c = 0; c < E; ++c) acc[c] *= fade;
-    const int runs = min(32, g1 - first + 1);
-    for (int i = 0; i < runs; i += 4) {                    // four runs' loads in flight
-      float part[4][E], wi[4], si[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        wi[k] = __shfl_sync(0xFFFFFFFFu, weight, (i + k) & 31);
-        si[k] = i + k < runs ? __shfl_sync(0xFFFFFFFFu, ml.y, (i + k) & 31) : 0.0f;
-        const int64_t at_k = __shfl_sync(0xFFFFFFFFu, slot, (i + k) & 31);
-        const float *src = p.part + at_k * D + lane * E;
-#pragma unroll
-        for (int c = 0; c < E; ++c) part[k][c] = si[k] != 0.0f ? src[c] : 0.0f;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (si[k] == 0.0f) continue;                    // nothing seen there
-        sum = fmaf(wi[k], si[k], sum);
-#pragma unroll
-        for (int c = 0; c < E; ++c) acc[c] = fmaf(wi[k], part[k][c], acc[c]);
-      }
-    }
-  }
+  if (!folds) return;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int c = 0; c < E; ++c) dst[c] = Elt<T>::from_float(acc[c] * inv);
@@ -243,12 +284,21 @@ template <int D> int launch_simt(const Params &p, cudaStream_t stream) {
   return LRQK_OK;
 }
 
-template <typename T, int D> int launch_combine(const Params &p, cudaStream_t stream) {
+template <typename T, int D, int WARPS> int combine_with(const Params &p, cudaStream_t stream) {
   const int64_t rows = (int64_t)p.batch * p.q_heads * p.nodes;
   // A plain launch: as a dependent one its CTAs sat beside the last products and the pair took 2 us longer.
-  tree_combine_kernel<T, D><<<(unsigned)ceil_div64(rows, 8), 256, 0, stream>>>(p);
+  tree_combine_kernel<T, D, WARPS><<<(unsigned)ceil_div64(rows, 8 / WARPS), 256, 0, stream>>>(p);
   LRQK_LAUNCH_CHECK();
   return LRQK_OK;
+}
+
+template <typename T, int D> int launch_combine(const Params &p, cudaStream_t stream) {
+  // at most so many runs share a unit (where all units are alike): eight to a warp, whose loads it has in flight at once
+  const int64_t units = (int64_t)p.batch * p.cache_heads, runs = p.groups / units + 2;
+  if (runs <= 8) return combine_with<T, D, 1>(p, stream);
+  if (runs <= 16) return combine_with<T, D, 2>(p, stream);
+  if (runs <= 32) return combine_with<T, D, 4>(p, stream);
+  return combine_with<T, D, 8>(p, stream);
 }
 
 // The split of these arguments (no device work).
