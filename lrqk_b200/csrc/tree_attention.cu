@@ -4,16 +4,18 @@
 // This file: the entry points, the fp32 kernel and the combine kernel.  (bf16 runs on the tensor cores,
 // tree_attention_tc.cu.)  One pass over the keys with a running maximum and sum; scores, weights and sums in fp32.
 //
-// The fp32 kernel keeps to fp32 multiply-adds (tf32 would cost three digits).  A CTA holds 64 query rows and walks 64-key
-// tiles: scores from 4 x 4 register tiles, weights through shared memory, 4 rows x head_dim/16 columns of the result in
-// registers.  Bound: fp32 FMA from about 16 rows a cache head on, HBM below.
+// The fp32 kernel keeps to fp32 multiply-adds (tf32 would cost three digits), packed two to an instruction.  A CTA holds 64
+// query rows and walks 32-key tiles: scores from 4 x 2 register tiles, weights through shared memory, 4 rows x head_dim/16
+// columns of the result in registers, the next tile's keys and values on their way in registers meanwhile.  75 KiB of
+// shared memory: two CTAs an SM (64-key tiles took 115 KiB, one CTA and twice the time).  Bound: shared-memory reads of the
+// register tiles.
 #include "tree_plan.cuh"
 
 namespace lrqk {
 namespace tree {
 namespace {
 
-constexpr int kRows = 64, kKeys = 64, kThreads = 256;
+constexpr int kRows = 64, kKeys = 32, kThreads = 256;
 
 // Two fp32 multiply-adds in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -24,11 +26,11 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 
 template <int D> struct SimtShared {
-  float q[kRows][D], k[kKeys][D + 4], v[kKeys][D], w[kRows][kKeys + 1];
+  float q[kRows][D], k[kKeys][D + 4], v[kKeys][D], w[kRows][kKeys + 4];
 };
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) tree_simt_kernel(const __grid_constant__ Params p) {
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -50,7 +52,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
       const int r = i / (D / VE), c = i % (D / VE) * VE;
       float f[VE] = {};
       if (r < n_rows) {
-        const int g = (row0 + r) / p.nodes, t = (row0 + r) % p.nodes;
+        const int g = group_row(p, row0 + r), t = row0 + r - g * p.nodes;
         Elt<T>::unpack(ld16(static_cast<const T *>(p.q) + w.b * p.q_stride[0] + (int64_t)(w.head * per_head + g) * p.q_stride[1] + t * p.q_stride[2] + c), f);
       }
 #pragma unroll
@@ -66,7 +68,10 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
       for (int c = 0; c < 2 * DC; ++c) acc[i][c] = make_float2(0.0f, 0.0f);
     }
     const int tree_head = w.head / (p.cache_heads / p.tree_heads);
-    for (int tile = w.t0; tile < w.t1; ++tile) {
+    // a tile's keys and values, into registers (rows behind the filled ones are never read: they may hold anything)
+    constexpr int kLoads = kKeys * (D / VE) / kThreads;
+    float4 nk[kLoads], nv[kLoads];
+    const auto fetch = [&](int tile) {
       const bool drafted = tile >= w.ctiles;
       const int first = (drafted ? tile - w.ctiles : tile) * kKeys;
       const int n_keys = min(kKeys, (drafted ? p.nodes : w.len) - first);
@@ -75,50 +80,57 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
       const T *gv = drafted ? static_cast<const T *>(p.tree_v) + w.b * p.tv_stride[0] + tree_head * p.tv_stride[1]
                             : static_cast<const T *>(p.cache_v) + w.b * p.cv_stride[0] + w.head * p.cv_stride[1];
       const int64_t sk = drafted ? p.tk_stride[2] : p.ck_stride[2], sv = drafted ? p.tv_stride[2] : p.cv_stride[2];
-      __syncthreads();
-      for (int i = tid; i < kKeys * (D / VE); i += kThreads) {
-        const int r = i / (D / VE), c = i % (D / VE) * VE;
-        float fk[VE] = {}, fv[VE] = {};
-        if (r < n_keys) {                               // rows behind the filled ones are never read: they may hold anything
-          Elt<T>::unpack(ld16(gk + (int64_t)(first + r) * sk + c), fk);
-          Elt<T>::unpack(ld16(gv + (int64_t)(first + r) * sv + c), fv);
-        }
 #pragma unroll
-        for (int j = 0; j < VE; ++j) { sm.k[r][c + j] = fk[j]; sm.v[r][c + j] = fv[j]; }
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = (tid + i * kThreads) / (D / VE), c = (tid + i * kThreads) % (D / VE) * VE;
+        nk[i] = nv[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < n_keys) {
+          nk[i] = *reinterpret_cast<const float4 *>(gk + (int64_t)(first + r) * sk + c);
+          nv[i] = *reinterpret_cast<const float4 *>(gv + (int64_t)(first + r) * sv + c);
+        }
+      }
+    };
+    fetch(w.t0);
+    for (int tile = w.t0; tile < w.t1; ++tile) {
+      const bool drafted = tile >= w.ctiles;
+      const int first = (drafted ? tile - w.ctiles : tile) * kKeys;
+      const int n_keys = min(kKeys, (drafted ? p.nodes : w.len) - first);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int r = (tid + i * kThreads) / (D / VE), c = (tid + i * kThreads) % (D / VE) * VE;
+        *reinterpret_cast<float4 *>(&sm.k[r][c]) = nk[i];
+        *reinterpret_cast<float4 *>(&sm.v[r][c]) = nv[i];
       }
       __syncthreads();
+      if (tile + 1 < w.t1) fetch(tile + 1);
       if (works) {                                      // whole half-warps: a row's 16 threads stay together
-        float2 s2[4][4] = {};                           // sums over even and odd columns
+        float2 s2[4][2] = {};                           // sums over even and odd columns
 #pragma unroll 4
         for (int c = 0; c < D; c += 4) {
-          float4 a[4], b[4];
+          float4 a[4], b[2];
 #pragma unroll
           for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4 *>(&sm.q[ty * 4 + i][c]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(&sm.k[tx + 16 * j][c]);
+          for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const float4 *>(&sm.k[tx + 16 * j][c]);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
               s2[i][j] = fma2(make_float2(a[i].x, a[i].y), make_float2(b[j].x, b[j].y),
                               fma2(make_float2(a[i].z, a[i].w), make_float2(b[j].z, b[j].w), s2[i][j]));
         }
-        float s[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[i][j] = s2[i][j].x + s2[i][j].y;
         const unsigned half = (tid & 16) ? 0xFFFF0000u : 0x0000FFFFu;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int r = row0 + ty * 4 + i, node = r % p.nodes;
-          float m = top[i];
+          const int r = row0 + ty * 4 + i, node = r - group_row(p, r) * p.nodes;
+          float m = top[i], s[2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 2; ++j) {
             const int key = tx + 16 * j;
             const bool seen = key < n_keys && r < p.rows && (!drafted || sees(p, w.b, node, first + key));
-            s[i][j] = seen ? s[i][j] * p.scale_log2 : -INFINITY;
-            m = fmaxf(m, s[i][j]);
+            s[j] = seen ? (s2[i][j].x + s2[i][j].y) * p.scale_log2 : -INFINITY;
+            m = fmaxf(m, s[j]);
           }
 #pragma unroll
           for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(half, m, o));
@@ -126,8 +138,8 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
           top[i] = m;
           float add = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float e = exp2f(s[i][j] - at);
+          for (int j = 0; j < 2; ++j) {
+            const float e = exp2f(s[j] - at);
             sm.w[ty * 4 + i][tx + 16 * j] = e;
             add += e;
           }
@@ -138,18 +150,26 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
           for (int c = 0; c < 2 * DC; ++c) acc[i][c] = make_float2(acc[i][c].x * fade, acc[i][c].y * fade);
         }
         __syncwarp(half);
-        for (int key = 0; key < n_keys; ++key) {
-          float4 v[DC];
+        // (rows of the tile behind the filled ones are zeros, their weights too)
+#pragma unroll 2
+        for (int key = 0; key < kKeys; key += 4) {
+          float4 e4[4];
 #pragma unroll
-          for (int c = 0; c < DC; ++c) v[c] = *reinterpret_cast<const float4 *>(&sm.v[key][tx * 4 + 64 * c]);
+          for (int i = 0; i < 4; ++i) e4[i] = *reinterpret_cast<const float4 *>(&sm.w[ty * 4 + i][key]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float e = sm.w[ty * 4 + i][key];
-            if (drafted && e == 0.0f) continue;         // a node that the row does not see adds nothing, whatever it holds
+          for (int k = 0; k < 4; ++k) {
+            float4 v[DC];
 #pragma unroll
-            for (int c = 0; c < DC; ++c) {
-              acc[i][2 * c] = fma2(make_float2(e, e), make_float2(v[c].x, v[c].y), acc[i][2 * c]);
-              acc[i][2 * c + 1] = fma2(make_float2(e, e), make_float2(v[c].z, v[c].w), acc[i][2 * c + 1]);
+            for (int c = 0; c < DC; ++c) v[c] = *reinterpret_cast<const float4 *>(&sm.v[key + k][tx * 4 + 64 * c]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float e = k == 0 ? e4[i].x : k == 1 ? e4[i].y : k == 2 ? e4[i].z : e4[i].w;
+              if (drafted && e == 0.0f) continue;       // a node that the row does not see adds nothing, whatever it holds
+#pragma unroll
+              for (int c = 0; c < DC; ++c) {
+                acc[i][2 * c] = fma2(make_float2(e, e), make_float2(v[c].x, v[c].y), acc[i][2 * c]);
+                acc[i][2 * c + 1] = fma2(make_float2(e, e), make_float2(v[c].z, v[c].w), acc[i][2 * c + 1]);
+              }
             }
           }
         }
@@ -161,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const __grid_consta
       const int r = row0 + ty * 4 + i;
       if (r >= p.rows) continue;
       if (w.whole()) {
-        const int g = r / p.nodes, t = r % p.nodes;
+        const int g = group_row(p, r), t = r - g * p.nodes;
         const int64_t at = ((int64_t)w.b * p.q_heads + w.head * per_head + g) * p.nodes + t;
         const float inv = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
         T *dst = static_cast<T *>(p.out) + at * D;
