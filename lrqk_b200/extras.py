@@ -27,6 +27,7 @@ import torch
 
 from .lrqk_attention import (DynamicLRQKCache, LightAttentionIndicesFactory, LightAttentionIndicesNoHitMiss,
                              _CacheBase)
+from .sampling import sample_tokens
 
 
 class LightAttentionIndicesOffloadPrefill(LightAttentionIndicesFactory):
@@ -63,6 +64,10 @@ class LightAttentionIndicesOffloadPrefill(LightAttentionIndicesFactory):
     def _decode(self, *args, **kwargs):
         self._restore()
         return super()._decode(*args, **kwargs)
+
+    def attend_tree(self, *args, **kwargs):
+        self._restore()
+        return super().attend_tree(*args, **kwargs)
 
 
 class _HostKV:
@@ -282,9 +287,10 @@ task_dict = {
 
 
 def tps_estimate(model, past_key_values_factory: Optional[Callable] = None, prompt_lens=(4096,), max_new_tokens: int = 32,
-                 vocab_size: Optional[int] = None, seed: int = 0) -> dict:
+                 vocab_size: Optional[int] = None, seed: int = 0, sampling: Optional[dict] = None) -> dict:
     """Prompt and decode tokens per second of greedy generation for each prompt length
-    (tps_estimate.py:41-85), on seeded uniform-random token ids."""
+    (tps_estimate.py:41-85), on seeded uniform-random token ids.  ``sampling``: settings of ``sample_tokens``
+    (temperature, top_k, top_p, min_p); tokens are then drawn with seeded random numbers instead."""
     wrapper, _ = WrapForwardTimer.wrap(model)
     vocab = vocab_size or model.config.vocab_size
     device = next(model.parameters()).device
@@ -293,15 +299,22 @@ def tps_estimate(model, past_key_values_factory: Optional[Callable] = None, prom
         for n in prompt_lens:
             g = torch.Generator().manual_seed(seed + n)
             ids = torch.randint(0, vocab, (1, n), generator=g).to(device)
+            draws = torch.Generator(device=device).manual_seed(seed + n)
+
+            def choose(logits):
+                if sampling is None:
+                    return logits.argmax(-1, keepdim=True)
+                return sample_tokens(logits, torch.rand(1, generator=draws, device=device), **sampling)[0].unsqueeze(1)
+
             wrapper.reset()
             cache = past_key_values_factory() if past_key_values_factory is not None else None
             with torch.no_grad():
                 logits = model(input_ids=ids, past_key_values=cache, use_cache=True)
                 cache = logits.past_key_values
-                tok = logits.logits[:, -1].argmax(-1, keepdim=True)
+                tok = choose(logits.logits[:, -1])
                 for _ in range(max_new_tokens):
                     res = model(input_ids=tok, past_key_values=cache, use_cache=True)
-                    tok = res.logits[:, -1].argmax(-1, keepdim=True)
+                    tok = choose(res.logits[:, -1])
             out[str(n)] = {"prefill_tps": wrapper.prefill_tps(), "decode_tps": wrapper.decode_tps()}
     finally:
         wrapper.remove_wrapper()
@@ -309,10 +322,10 @@ def tps_estimate(model, past_key_values_factory: Optional[Callable] = None, prom
 
 
 def run_task(name: str, model, *, r: int = 16, num_active_tokens: int = 1024, lite_tokens: int = 16, prompt_lens=(4096,),
-             max_new_tokens: int = 32, out_path: Optional[str] = None) -> dict:
+             max_new_tokens: int = 32, out_path: Optional[str] = None, sampling: Optional[dict] = None) -> dict:
     """One row of the reference's throughput table (tps_estimate.py:126-142): ``name`` in ``task_dict``.
     Like the reference's driver (:127-130), a row whose ``out_path`` already exists is not measured again: the
-    file's records are returned."""
+    file's records are returned.  ``sampling``: as for ``tps_estimate``."""
     if name not in task_dict:
         raise ValueError(f"Unknown task {name}")
     if out_path and os.path.exists(out_path):
@@ -328,7 +341,7 @@ def run_task(name: str, model, *, r: int = 16, num_active_tokens: int = 1024, li
         factory = lambda: DynamicLRQKCache(r=r, num_active_tokens=num_active_tokens, lite_tokens=lite_tokens,  # noqa: E731
                                            max_sequence_length=max(prompt_lens) + max_new_tokens + 64,
                                            num_key_value_groups=groups, lwattn_factory=cls)
-    records = tps_estimate(model, factory, prompt_lens=prompt_lens, max_new_tokens=max_new_tokens)
+    records = tps_estimate(model, factory, prompt_lens=prompt_lens, max_new_tokens=max_new_tokens, sampling=sampling)
     if out_path:
         with open(out_path, "w") as f:
             json.dump(records, f, indent=4)

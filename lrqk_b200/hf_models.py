@@ -31,6 +31,12 @@ each rank's cache holds its share of the (batch x KV head) units, the prompt's a
 for those heads only and all-gathered, and ``cache.attend`` returns all heads' rows through the
 exchange fused into the attention kernel.
 
+With ``cache.drafting(mask)`` open, a decoding layer takes several tokens a call -- a drafted tree -- and attends them
+with ``cache.attend_tree``; the states change when ``cache.accept`` decodes the tokens that were right.
+
+``patch_model(model, fused_rotary=True)`` rotates q and k of prompts and drafts with ``rotary.apply_rotary`` (one launch,
+angles right at far positions, one rounding) instead of the family's eager function; off, results are those of that function.
+
 Any other cache type falls through to the family's original forward.
 """
 from __future__ import annotations
@@ -44,6 +50,7 @@ import torch
 import torch.nn.functional as F
 
 from .lrqk_attention import DynamicLRQKCache
+from .rotary import apply_rotary
 
 SUPPORTED_FAMILIES = ("qwen", "llama", "mistral")
 
@@ -122,7 +129,7 @@ def lrqk_attention_forward(self, hidden_states: torch.Tensor,
     cache: DynamicLRQKCache = past_key_values
     input_shape = hidden_states.shape[:-1]
     hidden_shape = (*input_shape, -1, self.head_dim)
-    if hidden_states.shape[1] == 1 and cache.is_decoding(self.layer_idx):
+    if hidden_states.shape[1] == 1 and cache.is_decoding(self.layer_idx) and not cache.is_drafting:
         # decode step: one fused projection, then one kernel that rotates q and k and hands this rank's heads
         # to the layer step (instead of three projections and the dozen element-wise launches of the rotary op)
         fused = _fused_qkv(self)
@@ -140,14 +147,20 @@ def lrqk_attention_forward(self, hidden_states: torch.Tensor,
     key_states = self.k_proj(hidden_states).view(hidden_shape).transpose(1, 2)
     value_states = self.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
     cos, sin = position_embeddings
-    rope = sys.modules[type(self).__module__].apply_rotary_pos_emb
-    query_states, key_states = rope(query_states, key_states, cos, sin)
+    rotary, position_ids = getattr(self, "_lrqk_rotary", None), kwargs.get("position_ids")
+    if rotary is not None and position_ids is not None:
+        query_states, key_states = apply_rotary(query_states, key_states, position_ids, rotary[0], factor=rotary[1])
+    else:
+        rope = sys.modules[type(self).__module__].apply_rotary_pos_emb
+        query_states, key_states = rope(query_states, key_states, cos, sin)
 
     q_len = query_states.shape[2]
-    if cache.is_decoding(self.layer_idx):
+    if cache.is_decoding(self.layer_idx) and cache.is_drafting:
+        attn_output = cache.attend_tree(query_states, key_states, value_states, self.layer_idx).transpose(1, 2)
+    elif cache.is_decoding(self.layer_idx):
         if q_len != 1:
             raise NotImplementedError("a decoding LRQK layer takes one new token per call, like the reference's "
-                                      "LightAttentionIndicesFactory.decode")
+                                      "LightAttentionIndicesFactory.decode (several as a draft: DynamicLRQKCache.drafting)")
         attn_output = cache.attend(query_states, key_states, value_states, self.layer_idx).transpose(1, 2)
     else:
         pad = _padding_mask(attention_mask, key_states.shape[2])
@@ -244,7 +257,7 @@ def lrqk_decoder_layer_forward(self, hidden_states: torch.Tensor, attention_mask
     forward."""
     cache = past_key_values
     n1 = n2 = gate_up = None
-    if (isinstance(cache, DynamicLRQKCache) and hidden_states.shape[1] == 1 and cache.is_decoding(self.self_attn.layer_idx)
+    if (isinstance(cache, DynamicLRQKCache) and hidden_states.shape[1] == 1 and cache.is_decoding(self.self_attn.layer_idx) and not cache.is_drafting
             and _lrqk_dtype(hidden_states) is not None and hidden_states.is_contiguous()):
         n1, n2 = _norm_params(self.input_layernorm), _norm_params(self.post_attention_layernorm)
         gate_up = _fused_gate_up(self.mlp)
@@ -270,13 +283,26 @@ def family_of(model_name: str) -> str:
     raise ValueError(f"Unknown model name: {model_name}")
 
 
-def patch_model(model) -> int:
-    """Replace ``self_attn.forward`` of every decoder layer; returns the number of layers patched."""
+def _model_rotary(model):
+    """(inv_freq float64, factor) of a model's own rotary module, for the kinds whose frequencies do not change with the
+    sequence."""
+    module = getattr(model.model, "rotary_emb", None)
+    kind = getattr(module, "rope_type", None)
+    if kind not in ("default", "linear", "yarn", "llama3"):
+        raise ValueError(f"fused_rotary: rotary module of type {kind!r}; default, linear, yarn and llama3 have fixed frequencies")
+    return module.inv_freq.detach().double(), float(module.attention_scaling)
+
+
+def patch_model(model, fused_rotary: bool = False) -> int:
+    """Replace ``self_attn.forward`` of every decoder layer; returns the number of layers patched.  ``fused_rotary``:
+    prompts and drafts take ``apply_rotary`` with the model's own frequencies instead of the eager function."""
     n = 0
+    rotary = _model_rotary(model) if fused_rotary else None
     for layer in model.model.layers:
         attn = getattr(layer, "self_attn", None)
         if attn is None:
             continue
+        attn._lrqk_rotary = None if rotary is None else (rotary[0].to(attn.q_proj.weight.device), rotary[1])
         if not hasattr(attn, "_lrqk_original_forward"):
             attn._lrqk_original_forward = attn.forward
             attn.forward = types.MethodType(lrqk_attention_forward, attn)

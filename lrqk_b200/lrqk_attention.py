@@ -18,6 +18,7 @@ the constructors of the compute classes raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import enum
 from collections import defaultdict
@@ -27,6 +28,7 @@ import torch
 
 from . import _lib
 from .state import HostStore, LayerState, _ptr, _stream, on_device
+from .tree import tree_attention
 
 try:  # HF is only needed for the Cache base class
     from transformers import cache_utils as _cache_utils
@@ -704,6 +706,22 @@ class LightAttentionIndicesFactory:
         st = self._decode(query_states, key_states, value_states, attention=True, exchange=exchange)
         return st.attn_out.unsqueeze(2)
 
+    @torch.no_grad()
+    def attend_tree(self, query_states: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor,
+                    mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of T drafted tokens (query_states [B,Hq,T,d], key_states / value_states [B,Hkv,T,d], already at
+        their positions) over the resident rows as the last step left them and over the drafted tokens that each sees
+        (``tree.tree_attention``; ``mask`` as there).  Changes nothing: the layer selects, fetches and appends when a
+        token is decoded (or accepted).  Returns [B,Hq,T,d]."""
+        st = self.state
+        if st is None:
+            raise RuntimeError("attend_tree before prefill")
+        if query_states.device != st.device:
+            raise ValueError(f"this layer's state lives on {st.device}, the drafted tokens on {query_states.device}")
+        rows = min(self.current_len, self.gpu_capacity)
+        return tree_attention(query_states.to(st.dtype), st.K_res.narrow(2, 0, rows), st.V_res.narrow(2, 0, rows),
+                              key_states.to(st.dtype), value_states.to(st.dtype), mask)
+
     def miss_counts(self) -> torch.Tensor:
         """int32 [B,Hq]: slots refilled by the last step (device tensor; reading it synchronises)."""
         return self.state.miss_count
@@ -828,6 +846,8 @@ class DynamicLRQKCache(_CacheBase):
         self.temp_buff_cache_qkv: Dict[int, _CacheQKV] = defaultdict(lambda: _CacheQKV(num_active_tokens, 2))
         self.sequence_state = defaultdict(lambda: DynamicLRQKCache.State.pending)
         self.sharding = None
+        self._draft = None                                       # (mask,) while drafting() is open
+        self._drafted: Dict[int, tuple] = {}                     # q, k, v of the last draft, per layer
 
     def shard_heads(self, group=None, sharding=None):
         """Run every layer for this rank's share of the (batch x KV head) units only (one process per
@@ -933,6 +953,56 @@ class DynamicLRQKCache(_CacheBase):
         exchange = self.sharding.exchange(q.shape[0] * q.shape[1], q.shape[-1], fac.state.dtype)
         fac.decode_attend_push(q, k, v, exchange)
         return self.sharding.gather_step(bsz, kv_heads, q_heads).unsqueeze(2)
+
+    # ---- drafted tokens ---------------------------------------------------------------------------
+    # (The reference decodes one token a call, :1506-1613; this is what verifying a draft needs on top.)
+    @contextlib.contextmanager
+    def drafting(self, mask: Optional[torch.Tensor] = None):
+        """While this is open, a decoding layer takes several tokens a call as a drafted tree: the patched model's
+        forward (``input_ids`` [B,T], ``position_ids`` of the nodes' depths) attends them with ``attend_tree`` under
+        ``mask`` (``tree_mask(parents)``; ``None``: a chain) and changes no layer's state.  ``accept`` then takes the
+        tokens that were right."""
+        if self.sharding is not None:
+            raise NotImplementedError("drafted tokens on a head-sharded cache")
+        if self._draft is not None:
+            raise RuntimeError("a draft is open already")
+        self._draft, self._drafted = (mask,), {}
+        try:
+            yield self
+        finally:
+            self._draft = None
+
+    @property
+    def is_drafting(self) -> bool:
+        return self._draft is not None
+
+    def attend_tree(self, query_states: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int) -> torch.Tensor:
+        """Inside ``drafting``: the drafted tokens' attention rows [B,Hq,T,d] of one layer; keeps their q, k, v for
+        ``accept``."""
+        if self._draft is None:
+            raise RuntimeError("attend_tree() is only valid inside drafting()")
+        if self.sequence_state[layer_idx] != self.State.decoding:
+            raise RuntimeError("attend_tree() is only valid once the layer is decoding; use update() before")
+        out = self.lwattn[layer_idx].attend_tree(query_states, key_states, value_states, self._draft[0])
+        self._drafted[layer_idx] = (query_states, key_states, value_states)
+        return out
+
+    def accept(self, nodes) -> None:
+        """Decode the last draft's ``nodes`` (indices along one path from the root, the same for every sequence) into
+        every layer, in order, from the q, k, v of the drafting call: ring write, projection, selection and fetch as
+        for any decoded token, without a forward of the model.  The draft is used up."""
+        if self._draft is not None:
+            raise RuntimeError("accept() after drafting() is closed")
+        if not self._drafted:
+            raise RuntimeError("no drafted tokens to accept")
+        nodes = [int(i) for i in nodes]
+        t = next(iter(self._drafted.values()))[0].shape[2]
+        if any(not 0 <= i < t for i in nodes) or any(b <= a for a, b in zip(nodes, nodes[1:])):
+            raise ValueError(f"nodes {nodes}: ascending indices below {t} are expected")
+        for layer_idx, (q, k, v) in self._drafted.items():
+            for i in nodes:
+                self.lwattn[layer_idx]._decode(q[:, :, i:i + 1], k[:, :, i:i + 1], v[:, :, i:i + 1], attention=False)
+        self._drafted = {}
 
     def state_dict(self) -> dict:
         """The whole cache for ``load_state_dict``: every decoding layer's ``state_dict()`` and the prompt rows of
