@@ -61,12 +61,10 @@ struct SampleShared {
 
 template <typename T> struct SampKey;                  // order-preserving keys and back
 template <> struct SampKey<float> {
-  static constexpr uint32_t kTop = 0xFFFFFFFFu;
   __device__ static __forceinline__ uint32_t of(float f) { return order_key(f); }
   __device__ static __forceinline__ float value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 };
 template <> struct SampKey<__nv_bfloat16> {
-  static constexpr uint32_t kTop = 0xFFFFu;
   __device__ static __forceinline__ uint32_t of(float f) { return order_key(f) >> 16; }
   __device__ static __forceinline__ float value(uint32_t k) { return __uint_as_float((k & 0x8000u) ? (k ^ 0x8000u) << 16 : ~k << 16); }
 };
@@ -79,7 +77,7 @@ __device__ __forceinline__ void pack(__nv_bfloat16 *to, const float (&f)[8]) {  
   *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-struct Cut { uint32_t key, index; };                   // kept: larger keys, and this key up to this index
+struct Cut { float value; uint32_t index; };           // kept: larger logits, and equal ones up to this index
 
 template <typename T> struct Sampler {
   static constexpr int VE = Elt<T>::kPerVec, STEP = 32 * VE;
@@ -131,9 +129,7 @@ template <typename T> struct Sampler {
   }
 
   __device__ __forceinline__ bool inside(const Cut &c, float f, int at) const {
-    if (c.key == 0) return true;                       // (no cut yet)
-    const uint32_t k = SampKey<T>::of(f);
-    return k > c.key || (k == c.key && index_of(at) <= c.index);
+    return f > c.value || (f == c.value && index_of(at) <= c.index);
   }
 
   __device__ __forceinline__ unsigned long long entry(float f, int at) const {
@@ -239,12 +235,12 @@ template <typename T> struct Sampler {
   // Cut the tokens inside `cut` to those from the largest down to where the count (MASS: the mass) reaches its target.
   // lowest: the smallest candidate.  Returns -1; or, for a count whose tokens all fit the list, their number, and makes no cut.
   template <bool MASS> __device__ int narrow(Cut &cut, float lowest, unsigned long long count, double share) {
-    uint32_t khi = SampKey<T>::of(top), klo = max(SampKey<T>::of(lowest), cut.key);
+    uint32_t khi = SampKey<T>::of(top), klo = SampKey<T>::of(fmaxf(MASS ? fmaxf(lowest, dust) : lowest, cut.value));
     unsigned long long target, above, in;
     // level 0: bins by distance from the maximum.  (Halved, so that the range of any two floats is finite.)
-    const float half_top = 0.5f * top, range = half_top - 0.5f * SampKey<T>::value(klo);
-    const float per = (float)kSampBins / range;
-    const auto bin0 = [&](float f) { return min(kSampBins - 1, max(0, (int)((half_top - 0.5f * f) * per))); };
+    const float range = 0.5f * top - 0.5f * SampKey<T>::value(klo), per = (float)kSampBins / range;
+    const float slope = -0.5f * per, start = 0.5f * top * per;
+    const auto bin0 = [&](float f) { return min(kSampBins - 1, max(0, (int)fmaf(f, slope, start))); };
     clear();
     each([&](float f, int at) {
       if ((MASS ? f > dust : candidate(f)) && inside(cut, f, at)) {
@@ -269,19 +265,16 @@ template <typename T> struct Sampler {
     const Cut old = cut;
     if (khi != klo) {
       // keys that can lie in that bin (a little wider: the test itself is bin0)
-      const float slack = (fabsf(top) + 2.0f * range) * 0x1p-20f + 1e-37f, step = 2.0f * range / kSampBins;
+      const float slack = (fabsf(top) + 2.0f * range) * 0x1p-20f + 1e-35f, step = 2.0f * range / kSampBins;
       khi = min(khi, SampKey<T>::of(fminf(top, top - step * (float)b0 + slack)));
       if (b0 < kSampBins - 1) klo = max(klo, SampKey<T>::of(top - step * (float)(b0 + 1) - slack));
       if (klo > khi) klo = khi;
     }
-    const auto in_reach = [&](float f, int at) {
-      if (!candidate(f) || bin0(f) != b0) return false;
-      const uint32_t k = SampKey<T>::of(f);
-      return k <= khi && k >= klo && inside(old, f, at);
-    };
+    float from = SampKey<T>::value(klo), to = SampKey<T>::value(khi);
+    const auto in_reach = [&](float f, int at) { return f >= from && f <= to && bin0(f) == b0 && inside(old, f, at); };
     for (;;) {
       // at most so many tokens are in reach: all, if each weighs no less than the smallest key
-      const unsigned long long least = MASS ? weight(SampKey<T>::value(klo)) : 1ull;
+      const unsigned long long least = MASS ? weight(from) : 1ull;
       if (least && in / least <= kList / 2) {
         const int n = gather(in_reach);
         if (n >= 0) {
@@ -302,14 +295,15 @@ template <typename T> struct Sampler {
       in = sm.pick_in;
       khi -= sm.pick_bin << shift;
       klo = shift == 0 ? khi : khi - klo < (1u << shift) ? klo : khi - (1u << shift) + 1u;
+      from = SampKey<T>::value(klo);
+      to = SampKey<T>::value(khi);
     }
     // equal logits by the hundred: the need-th of them, in index order
-    const unsigned long long each_w = MASS ? weight(SampKey<T>::value(khi)) : 1ull;
+    const unsigned long long each_w = MASS ? weight(to) : 1ull;
     const unsigned long long ties = each_w ? in / each_w : 0ull, need = each_w ? (target - above + each_w - 1) / each_w : 1ull;
-    cut.index = khi == old.key ? old.index : 0xFFFFFFFFu;
-    cut.key = khi;
+    cut = Cut{to, to == old.value ? old.index : 0xFFFFFFFFu};
     if (need < ties) {
-      locate([&](float f, int at) -> unsigned long long { return SampKey<T>::of(f) == khi && candidate(f) && inside(old, f, at) ? 1ull : 0ull; },
+      locate([&](float f, int at) -> unsigned long long { return f == to && inside(old, f, at) ? 1ull : 0ull; },
              [&](unsigned long long) { return need - 1; },
              [&](uint32_t index, float, unsigned long long) {
                for (int c = 0; c < csize; ++c) *cluster.map_shared_rank(&sm.tie_index, c) = index;
@@ -333,8 +327,7 @@ template <typename T> struct Sampler {
       if (before < target && before + w >= target) { sm.pick_above = e; }
     }
     __syncthreads();
-    cut.key = (uint32_t)(sm.pick_above >> 32);
-    cut.index = 0xFFFFFFFFu - (uint32_t)sm.pick_above;
+    cut = Cut{value_of(sm.pick_above), 0xFFFFFFFFu - (uint32_t)sm.pick_above};
     __syncthreads();
   }
 
@@ -541,7 +534,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
       const double y = ((double)f - (double)high) / (double)t;
       if (p.logprobs) p.logprobs[row] = (float)(y - log((double)total * 0x1p-44));
     };
-    Cut cut{0u, 0xFFFFFFFFu};
+    Cut cut{-INFINITY, 0u};                            // all
     int n = -1;
     if (k > 0 && k < p.vocab) n = s.template narrow<false>(cut, low, (unsigned long long)k, 0.0);
     if (n >= 0) {
@@ -550,7 +543,7 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
       if (q < 1.0f) s.template narrow<true>(cut, low, 0ull, (double)q);
       s.locate(
           [&](float f, int at) -> unsigned long long {
-            if (!s.inside(cut, f, at)) return 0ull;
+            if (!(f > s.dust) || !s.inside(cut, f, at)) return 0ull;
             const unsigned long long w = s.weight(f);
             return w >= floor_w ? w : 0ull;
           },
