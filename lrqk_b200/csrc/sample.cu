@@ -100,6 +100,18 @@ template <typename T> struct Sampler {
     for (int i = lane; i < p.chunk; i += 32) vals[warp * p.chunk + i] = Elt<T>::from_float(fn(Elt<T>::to_float(vals[warp * p.chunk + i])));
   }
 
+  // fn(values, place of the first in the slice) for this warp's chunk: four neighbours at a time
+  template <typename F> __device__ __forceinline__ void each4(F fn) const {
+    const int base = warp * p.chunk;
+    for (int s = 0; s < p.chunk; s += STEP) {
+      const int at = base + s + lane * VE;
+      float f[VE];
+      Elt<T>::unpack(ld16(vals + at), f);
+#pragma unroll
+      for (int j = 0; j < VE; j += 4) fn(f + j, at + j);
+    }
+  }
+
   // fn(value, place in the slice) for this warp's chunk, a lane's VE neighbours at a time
   template <typename F> __device__ __forceinline__ void each(F fn) const {
     const int base = warp * p.chunk;
@@ -116,8 +128,7 @@ template <typename T> struct Sampler {
 
   // round(2^44 exp((f - top) / T)), f <= top
   __device__ __forceinline__ unsigned long long weight(float f) const {
-    if (!(f > dust)) return 0ull;
-    const double y = ((double)f - (double)top) * per_log; // 128ths of an octave, above -6100
+    const double y = ((double)f - (double)top) * per_log; // 128ths of an octave, above -6100 where it counts
     const double magic = 6755399441055744.0;              // 1.5 * 2^52: the sum's low bits are the nearest whole number
     const double n = y + magic;
     const int k = __double2loint(n);
@@ -125,7 +136,8 @@ template <typename T> struct Sampler {
     const double e = fma(r, fma(r, fma(r, fma(r, 3.583032305400251e-11, 2.6466421444330967e-08), 1.4662262387640423e-05), 0.0054152123481245725), 1.0) * sm.table[k & (kTable - 1)];
     const double scaled = __hiloint2double(__double2hiint(e) + (((k >> 7) + kFracBits) << 20), __double2loint(e));
     const double whole = scaled + 4503599627370496.0;     // 2^52
-    return ((unsigned long long)(uint32_t)(__double2hiint(whole) - 0x43300000) << 32) | (uint32_t)__double2loint(whole);
+    const unsigned long long w = ((unsigned long long)(uint32_t)(__double2hiint(whole) - 0x43300000) << 32) | (uint32_t)__double2loint(whole);
+    return f > dust ? w : 0ull;                           // (no branch: neighbours' chains of double operations overlap)
   }
 
   __device__ __forceinline__ bool inside(const Cut &c, float f, int at) const {
@@ -242,11 +254,13 @@ template <typename T> struct Sampler {
     const float slope = -0.5f * per, start = 0.5f * top * per;
     const auto bin0 = [&](float f) { return min(kSampBins - 1, max(0, (int)fmaf(f, slope, start))); };
     clear();
-    each([&](float f, int at) {
-      if ((MASS ? f > dust : candidate(f)) && inside(cut, f, at)) {
-        const unsigned long long w = MASS ? weight(f) : 1ull;
-        if (w) add<MASS>(bin0(f), w);
-      }
+    each4([&](const float *f, int at) {
+      unsigned long long w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = MASS ? weight(f[j]) : candidate(f[j]) ? 1ull : 0ull;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (w[j] && inside(cut, f[j], at + j)) add<MASS>(bin0(f[j]), w[j]);
     });
     const auto first_target = [&](unsigned long long total) {
       if (!MASS) return min(count, total);             // fewer candidates than asked for: all of them
@@ -377,7 +391,12 @@ template <typename T> struct Sampler {
   // is called by one thread of the cluster.
   template <typename W, typename G, typename F> __device__ void locate(W weigh, G target_of, F found) {
     unsigned long long mine = 0;
-    each([&](float f, int at) { mine += weigh(f, at); });
+    each4([&](const float *f, int at) {
+      unsigned long long w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = weigh(f[j], at + j);
+      mine += (w[0] + w[1]) + (w[2] + w[3]);
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
     if (lane == 0) sm.wsum[warp] = mine;
@@ -543,9 +562,8 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
       if (q < 1.0f) s.template narrow<true>(cut, low, 0ull, (double)q);
       s.locate(
           [&](float f, int at) -> unsigned long long {
-            if (!(f > s.dust) || !s.inside(cut, f, at)) return 0ull;
             const unsigned long long w = s.weight(f);
-            return w >= floor_w ? w : 0ull;
+            return w >= floor_w && s.inside(cut, f, at) ? w : 0ull;
           },
           target_of, found);
     }
