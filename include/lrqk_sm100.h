@@ -395,8 +395,8 @@ int lrqk_rotary(const lrqk_rotary_args *a, lrqk_stream_t stream);
  * one call.  Node i of sequence b attends to rows [0, cache_lens[b]) of the cache and to the drafted nodes j with
  * mask[b][i][j] != 0.  Changes no cache.
  *   q [batch, q_heads, nodes, d], cache_k / cache_v [batch, cache_heads, capacity, d], tree_k / tree_v [batch,
- *   tree_heads, nodes, d]: strides in elements (batch, head, row; 0 allowed), last dimension dense, every row on 16
- *   bytes.  tree_heads divides cache_heads divides q_heads: the resident rows of a decoding layer have cache_heads =
+ *   tree_heads, nodes, d]: strides in elements (batch, head, row; 0 allowed for batch and head), last dimension dense,
+ *   every row on 16 bytes.  tree_heads divides cache_heads divides q_heads: the resident rows of a decoding layer have cache_heads =
  *   q_heads, an ordinary cache cache_heads = tree_heads = the KV heads.
  *   cache_lens : device int32 [batch], read when the kernel runs and cut to [0, capacity]; NULL: capacity.  Rows behind
  *                a length are not used and may hold anything, as may nodes that no node sees.

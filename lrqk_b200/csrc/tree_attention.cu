@@ -392,6 +392,7 @@ int lrqk_tree_attention(const lrqk_tree_args *a, void *workspace, lrqk_stream_t 
     t.to[1] = t.heads > 1 ? t.from[1] : 0;
     t.to[2] = t.rows > 1 ? t.from[2] : 0;
     if (t.to[0] < 0 || t.to[1] < 0 || t.to[2] < 0) return LRQK_EINVAL;
+    if (t.rows > 1 && t.to[2] == 0) return LRQK_EINVAL;   // (a tensor copy cannot repeat one row)
     low |= (uintptr_t)((t.to[0] | t.to[1] | t.to[2]) * (int64_t)elt_size(a->dtype));
   }
   if (low & 15 || (reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(workspace)) & 31) return LRQK_EUNSUPPORTED;

@@ -916,6 +916,7 @@ class DynamicLRQKCache(_CacheBase):
                layer_idx: int, attention_mask: Optional[torch.Tensor] = None):
         if any(c is None for c in (query_states, key_states, value_states)):
             raise ValueError("None of query_states, key_states, and value_states can be None")
+        self._drafted = {}
         if self.sharding is not None:
             query_states, key_states, value_states, attention_mask = self._local(query_states, key_states,
                                                                                  value_states, attention_mask)
@@ -926,6 +927,7 @@ class DynamicLRQKCache(_CacheBase):
     def attend(self, query_states: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor,
                layer_idx: int) -> torch.Tensor:
         """Decode-state only: one step plus attention, returns [B,Hq,1,d]."""
+        self._drafted = {}                                       # a draft made before this token no longer follows the context
         if self.sequence_state[layer_idx] != self.State.decoding:
             raise RuntimeError("attend() is only valid once the layer is decoding; use update() before")
         fac = self.lwattn[layer_idx]
@@ -942,6 +944,7 @@ class DynamicLRQKCache(_CacheBase):
         """``attend`` from the fused projection of the new token: qkv [B, 1, (q_heads + 2 kv_heads) d] holds the
         un-rotated q, k and v heads of the whole model, cos / sin [B or 1, 1, d] the position's rotary factors.
         One kernel rotates q and k and cuts out this rank's heads; returns the rows of all heads [B,Hq,1,d]."""
+        self._drafted = {}
         if self.sequence_state[layer_idx] != self.State.decoding:
             raise RuntimeError("attend_qkv() is only valid once the layer is decoding; use update() before")
         fac, bsz = self.lwattn[layer_idx], qkv.shape[0]
@@ -969,6 +972,9 @@ class DynamicLRQKCache(_CacheBase):
         self._draft, self._drafted = (mask,), {}
         try:
             yield self
+        except BaseException:
+            self._drafted = {}                                   # some layers only: nothing to accept
+            raise
         finally:
             self._draft = None
 
@@ -1064,6 +1070,7 @@ class DynamicLRQKCache(_CacheBase):
             self._free()
 
     def _free(self):
+        self._drafted = {}
         for fac in self.lwattn.values():
             fac.close()
         if self.sharding is not None:

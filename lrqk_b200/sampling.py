@@ -23,7 +23,7 @@ def _setting(value: Setting, name: str, rows: int, device: torch.device, dtype: 
         return value.data_ptr(), 0
     if not math.isfinite(value) or value < low:
         raise ValueError(f"{name} must be finite and at least {low}, got {value}")
-    return None, value
+    return None, (min(value, 2 ** 31 - 1) if dtype is torch.int32 else value)
 
 
 def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0, top_k: Setting = 0, top_p: Setting = 1.0,
@@ -37,7 +37,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting
     probability exceeds ``u``.  The log-probability is that of the distribution the token was drawn from.
 
     Each setting is a number or a tensor [B] on the device (float32; ``top_k`` int32), read when the kernel runs.  NaN
-    logits count as -inf; a row without any logit above -inf gives token -1 and NaN."""
+    logits count as -inf; a row without any logit above -inf gives token -1 and NaN.  Nothing here has a gradient."""
     if logits.dim() != 2 or logits.dtype not in _DTYPES or not logits.is_cuda or logits.shape[1] == 0:
         raise ValueError(f"logits: expected a float32 or bfloat16 CUDA tensor [rows, vocab], got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
     rows, vocab = logits.shape

@@ -85,7 +85,7 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
       ``h // (Hq / Ht)``
     * ``scale``: default ``d ** -0.5``; T up to 256, d 64 or 128, float32 or bfloat16
 
-    Strided inputs are read as they are as long as rows are dense and start on 16 bytes.  Inference only (no gradient).
+    Strided inputs (and expanded batches and heads) are read as they are as long as rows are dense and start on 16 bytes.  Inference only (no gradient).
     Returns [B, Hq, T, d], with ``return_lse`` also the fp32 [B, Hq, T] natural log-sum-exp; a row that sees nothing gives
     zeros and -inf."""
     if q.dim() != 4 or q.dtype not in _DTYPES or not q.is_cuda:
@@ -111,6 +111,8 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     qs, ks, vs, tks, tvs = q.stride(), cache_k.stride(), cache_v.stride(), tree_k.stride(), tree_v.stride()
     if not qs[3] == ks[3] == vs[3] == tks[3] == tvs[3] == 1:
         raise ValueError("q, cache_k, cache_v, tree_k, tree_v: rows must be dense (last stride 1)")
+    if (cap > 1 and not (ks[2] and vs[2])) or (t > 1 and not (qs[2] and tks[2] and tvs[2])):
+        raise ValueError("q, cache_k, cache_v, tree_k, tree_v: one row expanded to many is not supported")
     mask_at = lens_at = lse_at = None
     mask_stride = 0
     if mask is not None:

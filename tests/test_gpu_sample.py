@@ -217,6 +217,7 @@ def test_refusals():
         a.update(kw)
         with pytest.raises(ValueError):
             sample_tokens(a.pop("logits"), a.pop("u"), **a)
+    assert torch.equal(sample_tokens(logits, u, top_k=2 ** 40)[0], sample_tokens(logits, u)[0])
     from lrqk_b200._lib import LrqkError
     with pytest.raises(LrqkError):
         sample_tokens(torch.zeros(1, 500000, device="cuda"), u[:1])

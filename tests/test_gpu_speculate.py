@@ -137,6 +137,18 @@ def test_draft_protocol_is_checked():
     cache.accept([0, 1])
     with pytest.raises(RuntimeError):
         cache.accept([0])
+    with torch.no_grad():
+        with cache.drafting():
+            model(input_ids=ids[:, :3], past_key_values=cache, use_cache=True)
+        model(input_ids=ids[:, :1], past_key_values=cache, use_cache=True)   # a token decoded in between
+        with pytest.raises(RuntimeError):
+            cache.accept([0])
+        with pytest.raises(KeyError):
+            with cache.drafting():
+                model(input_ids=ids[:, :3], past_key_values=cache, use_cache=True)
+                raise KeyError
+        with pytest.raises(RuntimeError):
+            cache.accept([0])                                          # a draft that was broken off
     cache.close()
 
 

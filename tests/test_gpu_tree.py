@@ -255,6 +255,10 @@ def test_refusals():
         tree_attention(*make(1, 2, 1, 1, 257, 8, 64, torch.bfloat16)[:5])
     with pytest.raises(ValueError):
         tree_attention(*make(1, 2, 1, 1, 3, 8, 96, torch.bfloat16)[:5])
+    one = ck[:, :, :1].expand(2, 2, 30, 64)                            # one row for all: a tensor copy cannot repeat it
+    for a in ((q, one, cv, tk, tv), (q, ck, one, tk, tv), (q, ck, cv, tk[:, :, :1].expand(2, 2, 5, 64), tv), (q[:, :, :1].expand(2, 4, 5, 64), ck, cv, tk, tv)):
+        with pytest.raises(ValueError):
+            tree_attention(*a)
     grad = q.float().requires_grad_()
     with pytest.raises(ValueError):
         tree_attention(grad, ck.float(), cv.float(), tk.float(), tv.float())
