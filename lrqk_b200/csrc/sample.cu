@@ -249,10 +249,12 @@ template <typename T> struct Sampler {
   template <bool MASS> __device__ int narrow(Cut &cut, float lowest, unsigned long long count, double share) {
     uint32_t khi = SampKey<T>::of(top), klo = SampKey<T>::of(fmaxf(MASS ? fmaxf(lowest, dust) : lowest, cut.value));
     unsigned long long target, above, in;
-    // level 0: bins by distance from the maximum.  (Halved, so that the range of any two floats is finite.)
+    // Level 0: bins by distance from the maximum.  (Halved, so that the range of any two floats is finite.)  The bin is the
+    // low bits of a sum with 2^23: a conversion instruction has a quarter of the rate.  `start` is rounded with it, to half a
+    // bin, alike for all logits.
     const float range = 0.5f * top - 0.5f * SampKey<T>::value(klo), per = (float)kSampBins / range;
-    const float slope = -0.5f * per, start = 0.5f * top * per;
-    const auto bin0 = [&](float f) { return min(kSampBins - 1, max(0, (int)fmaf(f, slope, start))); };
+    const float slope = -0.5f * per, start = 0.5f * top * per + 8388608.0f;
+    const auto bin0 = [&](float f) { return min(kSampBins - 1, max(0, __float_as_int(fmaf(f, slope, start)) - 0x4B000000)); };
     clear();
     each4([&](const float *f, int at) {
       unsigned long long w[4];
@@ -272,19 +274,19 @@ template <typename T> struct Sampler {
     above = sm.pick_above;
     in = sm.pick_in;
     target = first_target(sm.pick_total);
-    if (!MASS && above + in <= kList / 2) {
-      const int n = gather([&](float f, int at) { return candidate(f) && bin0(f) <= b0; });
-      if (n >= 0) return n;
-    }
     const Cut old = cut;
     if (khi != klo) {
-      // keys that can lie in that bin (a little wider: the test itself is bin0)
+      // keys that can lie in that bin (wider by a bin on either side, and some rounding: the test itself is bin0)
       const float slack = (fabsf(top) + 2.0f * range) * 0x1p-20f + 1e-35f, step = 2.0f * range / kSampBins;
-      khi = min(khi, SampKey<T>::of(fminf(top, top - step * (float)b0 + slack)));
-      if (b0 < kSampBins - 1) klo = max(klo, SampKey<T>::of(top - step * (float)(b0 + 1) - slack));
+      khi = min(khi, SampKey<T>::of(fminf(top, top - step * (float)(b0 - 1) + slack)));
+      if (b0 < kSampBins - 1) klo = max(klo, SampKey<T>::of(top - step * (float)(b0 + 2) - slack));
       if (klo > khi) klo = khi;
     }
     float from = SampKey<T>::value(klo), to = SampKey<T>::value(khi);
+    if (!MASS && above + in <= kList / 2) {
+      const int n = gather([&](float f, int at) { return f >= from && bin0(f) <= b0; });
+      if (n >= 0) return n;
+    }
     const auto in_reach = [&](float f, int at) { return f >= from && f <= to && bin0(f) == b0 && inside(old, f, at); };
     for (;;) {
       // at most so many tokens are in reach: all, if each weighs no less than the smallest key
@@ -572,12 +574,14 @@ __global__ void __launch_bounds__(kSampThreads, 2) sample_kernel(const __grid_co
 }
 
 template <typename T> int launch_sample(SampleParams &p, int rows, cudaStream_t stream) {
-  // Few rows: 8 CTAs each, for latency; more: fewer, as long as a slice fits.
+  // As many CTAs a row as two an SM can hold, for the passes over its slice are what takes the time: 25 rows of 128256 bf16
+  // logits take 51 us with 8 and 72 with 4, 64 rows of 152064 fp32 logits 71 with 8 and 81 with 4.  Fewer for many rows, as
+  // long as a slice fits.
   constexpr int step = 32 * Elt<T>::kPerVec * kSampWarps;       // a slice is a whole number of these
   int csize = 1;
   const auto slice = [&](int c) { return ceil_div64(ceil_div64(p.vocab, c), step) * step; };
   while (csize < kSampMaxCluster && (slice(csize) * (int64_t)sizeof(T) > (int64_t)kSampSliceBytes ||
-                                     (rows * csize <= kNumSMs && slice(csize) > step)))
+                                     (rows * csize <= 2 * kNumSMs && slice(csize) > step)))
     csize *= 2;
   if (slice(csize) * (int64_t)sizeof(T) > (int64_t)kSampSliceBytes) return LRQK_EUNSUPPORTED;
   p.chunk = (int)(slice(csize) / kSampWarps);

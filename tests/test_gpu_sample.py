@@ -147,6 +147,15 @@ def test_infinities_nan_and_extreme_ranges(dtype):
     assert tok[1] == -1 and tok[2] == -1 and bool(torch.isnan(lp[1:3]).all()) and tok[6] == 1234 and float(lp[6]) == 0.0
 
 
+@pytest.mark.parametrize("offset", [1e3, 3e4, -5e5])
+def test_logits_far_from_zero(offset):
+    """A spread of a few units on a large offset: fp32 logits a few hundredths apart at best, many of them equal."""
+    logits, u = make(8, 20000, torch.float32, 21)
+    l = logits + offset
+    for f in (dict(k=50), dict(p=0.9), dict(k=3000, p=0.6), dict(m=0.01), dict(t=0.02, p=0.99), dict()):
+        check(l, u, **f)
+
+
 @pytest.mark.parametrize("dtype", DT)
 def test_random_numbers_at_the_ends(dtype):
     logits, _ = make(6, 5000, dtype, 6)
