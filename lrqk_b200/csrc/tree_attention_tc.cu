@@ -15,7 +15,9 @@
 //
 // Warp 0 issues the copies (a ring of K and V tiles, 128-byte swizzle), warp 1 owns TMEM and issues the products, warps
 // 2.. form the weights: a warp has 32 rows and one half of a tile's keys.  The maximum in use of a row passes from one half
-// to the next (of this tile, of the next one): each adds its own keys' before it forms its weights.
+// to the next (of this tile, of the next one).  The second half does not wait for the first: it forms its weights against
+// the maximum it knows and looks afterwards whether the first half moved it, in which case it forms them again (rarely).
+// Waiting ahead of the weights cost the two-block kernel 13 % of its time.
 //
 // V rows behind a length may hold anything, and 0 * NaN is NaN: the softmax warps clear them in shared memory before the
 // product.  In a drafted tile, values of V out of range are replaced by zeros and their nodes noted; a row that sees such
@@ -521,36 +523,69 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             hide(u, drafted ? seen[1] : n >= 64 ? 0xFFFFFFFFu : n > 32 ? (1u << (n - 32)) - 1u : 0u);
           }
           const float now = fmaxf(max32(v), max32(u)) * p.scale_log2;
-          // the maximum in use, from the half before
-          float old = top;
-          if (half == 1 || cnt > 0) {
-            if (!await(&bar.decided[m][half ^ 1][quarter], (half == 1 ? cnt : cnt - 1) & 1)) { quit(); break; }
+          const float old = top;
+          const auto grown = [&](float in_use) { return now > in_use + kGrow || (in_use == -INFINITY && now > -INFINITY); };
+          // the second half goes ahead unless it would move the maximum itself, or knows none yet
+          const bool ahead = half == 1 && st > 0 && !__any_sync(0xFFFFFFFFu, grown(top));
+          if (ahead) {
+            // (with one row block the first half may be a tile ahead and move the maximum again: not before this half has looked)
+            if constexpr (MT == 2) signal(&bar.decided[m][1][quarter]);
+          } else {
+            // the maximum in use, from the half before (with two row blocks the scores of a tile follow its products: known)
+            if (half == 1 || (MT == 1 && cnt > 0)) {
+              if (!await(&bar.decided[m][half ^ 1][quarter], (half == 1 ? cnt : cnt - 1) & 1)) { quit(); break; }
+            }
             if (half == 1 || st > 0) top = bar.top[m][r_in];
-          }
-          const bool move = now > top + kGrow || (top == -INFINITY && now > -INFINITY);
-          const float use = move ? now : top;
-          if (move || (half == 0 && st == 0)) bar.top[m][r_in] = use;
-          signal(&bar.decided[m][half][quarter]);
-          if (__any_sync(0xFFFFFFFFu, move) && (half == 1 || st > 0)) {
-            // O holds the products up to the half before: that one has to be in it
-            const int px = MT == 1 ? (half == 1 ? x : x ^ 1) : m, pc = half == 1 ? cnt : cnt - 1;
-            if (!await(&bar.o_done[px][half ^ 1], (MT == 1 ? pc >> 1 : pc) & 1)) { quit(); break; }
-            fence_after();
-            const float fade = move ? exp2_fast(top - use) : 1.0f;
+            const bool move = grown(top);
+            const float use = move ? now : top;
+            if (move || (half == 0 && st == 0)) bar.top[m][r_in] = use;
+            signal(&bar.decided[m][half][quarter]);
+            if (__any_sync(0xFFFFFFFFu, move) && (half == 1 || st > 0)) {
+              // O holds the products up to the half before: that one has to be in it
+              const int px = MT == 1 ? (half == 1 ? x : x ^ 1) : m, pc = half == 1 ? cnt : cnt - 1;
+              if (!await(&bar.o_done[px][half ^ 1], (MT == 1 ? pc >> 1 : pc) & 1)) { quit(); break; }
+              fence_after();
+              const float fade = move ? exp2_fast(top - use) : 1.0f;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 8) scale8(o_base + c, fade);
+              for (int c = 0; c < D; c += 8) scale8(o_base + c, fade);
+            }
+            top = use;
           }
-          top = use;
           if (old != top) sum *= exp2_fast(old - top);
-          const uint64_t c2 = pair(p.scale_log2, p.scale_log2), minus2 = top == -INFINITY ? 0 : pair(-top, -top);
+          const uint64_t c2 = pair(p.scale_log2, p.scale_log2);
           uint64_t sum2 = 0;
-          weigh(v, c2, minus2, sum2);
+          {
+            const uint64_t minus2 = top == -INFINITY ? 0 : pair(-top, -top);
+            weigh(v, c2, minus2, sum2);
+            weigh(u, c2, minus2, sum2);
+          }
+          if (ahead) {
+            if (!await(&bar.decided[m][0][quarter], cnt & 1)) { quit(); break; }
+            const float first = bar.top[m][r_in];
+            if constexpr (MT == 1) signal(&bar.decided[m][1][quarter]);
+            if (__any_sync(0xFFFFFFFFu, first != top)) {  // the first half moved it: again, from the scores in TMEM
+              if (first != top) sum *= exp2_fast(top - first);
+              top = first;
+              load32_async(s_base, v);
+              load32_async(s_base + 32, u);
+              load_wait();
+              pin(v);
+              pin(u);
+              if (masked) {
+                const int n = n_keys - half * 64;
+                hide(v, drafted ? seen[0] : n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u);
+                hide(u, drafted ? seen[1] : n >= 64 ? 0xFFFFFFFFu : n > 32 ? (1u << (n - 32)) - 1u : 0u);
+              }
+              const uint64_t minus2 = top == -INFINITY ? 0 : pair(-top, -top);
+              sum2 = 0;
+              weigh(v, c2, minus2, sum2);
+              weigh(u, c2, minus2, sum2);
+            }
+          }
           if constexpr (MT == 1) {
             store_two_parts(v, s_base);
-            weigh(u, c2, minus2, sum2);
             store_two_parts(u, s_base + 32);
           } else {
-            weigh(u, c2, minus2, sum2);
             uint32_t o[32];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
