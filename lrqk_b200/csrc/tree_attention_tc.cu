@@ -15,9 +15,9 @@
 //
 // Warp 0 issues the copies (a ring of K and V tiles, 128-byte swizzle), warp 1 owns TMEM and issues the products, warps
 // 2.. form the weights: a warp has 32 rows and one half of a tile's keys.  The maximum in use of a row passes from one half
-// to the next (of this tile, of the next one).  The second half does not wait for the first: it forms its weights against
-// the maximum it knows and looks afterwards whether the first half moved it, in which case it forms them again (rarely).
-// Waiting ahead of the weights cost the two-block kernel 13 % of its time.
+// to the next (of this tile, of the next one).  With two row blocks the second half does not wait for the first: it forms its
+// weights against the maximum it knows and looks afterwards whether the first half moved it, in which case it forms them
+// again (rarely); waiting ahead of the weights cost that kernel a fifth of its time.
 //
 // V rows behind a length may hold anything, and 0 * NaN is NaN: the softmax warps clear them in shared memory before the
 // product.  In a drafted tile, values of V out of range are replaced by zeros and their nodes noted; a row that sees such
@@ -525,11 +525,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           const float now = fmaxf(max32(v), max32(u)) * p.scale_log2;
           const float old = top;
           const auto grown = [&](float in_use) { return now > in_use + kGrow || (in_use == -INFINITY && now > -INFINITY); };
-          // the second half goes ahead unless it would move the maximum itself, or knows none yet
-          const bool ahead = half == 1 && st > 0 && !__any_sync(0xFFFFFFFFu, grown(top));
+          // the second half of two row blocks goes ahead unless it would move the maximum itself, or knows none yet.  (With one
+          // row block the first half may be a tile ahead and move the maximum again before this one has looked.)
+          const bool ahead = MT == 2 && half == 1 && st > 0 && !__any_sync(0xFFFFFFFFu, grown(top));
           if (ahead) {
-            // (with one row block the first half may be a tile ahead and move the maximum again: not before this half has looked)
-            if constexpr (MT == 2) signal(&bar.decided[m][1][quarter]);
+            signal(&bar.decided[m][1][quarter]);
           } else {
             // the maximum in use, from the half before (with two row blocks the scores of a tile follow its products: known)
             if (half == 1 || (MT == 1 && cnt > 0)) {
@@ -562,7 +562,6 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           if (ahead) {
             if (!await(&bar.decided[m][0][quarter], cnt & 1)) { quit(); break; }
             const float first = bar.top[m][r_in];
-            if constexpr (MT == 1) signal(&bar.decided[m][1][quarter]);
             if (__any_sync(0xFFFFFFFFu, first != top)) {  // the first half moved it: again, from the scores in TMEM
               if (first != top) sum *= exp2_fast(top - first);
               top = first;
