@@ -92,11 +92,16 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
         raise ValueError(f"q: expected a float32 or bfloat16 CUDA tensor [batch, heads, nodes, head_dim], got {q.dtype} {tuple(q.shape)} on {q.device}")
     b, hq, t, d = q.shape
     device, dtype = q.device, q.dtype
-    hc, cap, ht = cache_k.shape[1], cache_k.shape[2], tree_k.shape[1]
-    for name, x, shape in (("cache_k", cache_k, (b, hc, cap, d)), ("cache_v", cache_v, (b, hc, cap, d)), ("tree_k", tree_k, (b, ht, t, d)),
-                           ("tree_v", tree_v, (b, ht, t, d))):
-        if x.shape != shape or x.dtype is not dtype or x.device != device:
-            raise ValueError(f"{name}: expected {dtype} {list(shape)} on {device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    if cache_k.dim() != 4 or tree_k.dim() != 4:
+        raise ValueError(f"cache_k, tree_k: expected [{b}, heads, rows, {d}], got {tuple(cache_k.shape)}, {tuple(tree_k.shape)}")
+    cb, hc, cap, cd = cache_k.shape
+    tb, ht, tt, td = tree_k.shape
+    if not (cb == tb == b and cd == td == d and tt == t and cache_v.shape == cache_k.shape and tree_v.shape == tree_k.shape
+            and cache_k.dtype is dtype and cache_v.dtype is dtype and tree_k.dtype is dtype and tree_v.dtype is dtype
+            and cache_k.device == device and cache_v.device == device and tree_k.device == device and tree_v.device == device):
+        raise ValueError(f"cache_k, cache_v: expected {dtype} [{b}, cache heads, rows, {d}], tree_k, tree_v: [{b}, tree heads, {t}, {d}], all on {device}; got "
+                         + ", ".join(f"{n} {x.dtype} {tuple(x.shape)} on {x.device}"
+                                     for n, x in (("cache_k", cache_k), ("cache_v", cache_v), ("tree_k", tree_k), ("tree_v", tree_v))))
     if hc == 0 or ht == 0 or hq == 0 or hq % hc or hc % ht:
         raise ValueError(f"heads: tree heads divide cache heads divide query heads; got q {hq}, cache {hc}, tree {ht}")
     if t > MAX_NODES:
@@ -136,7 +141,7 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
                           tree_k.data_ptr(), tree_v.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
                           tks[0], tks[1], tks[2], tvs[0], tvs[1], tvs[2], lens_at, mask_at, mask_stride, out.data_ptr(), lse_at,
                           _status_word(device))
-        ws = torch.empty((lib.lrqk_tree_attention_workspace_bytes(a),), dtype=torch.uint8, device=device)
+        ws = torch.empty(lib.lrqk_tree_attention_workspace_bytes(a), dtype=torch.uint8, device=device)
         code = call_on(device, lib.lrqk_tree_attention, a, ws.data_ptr())
         if code == _lib.EUNSUPPORTED:
             _refuse_rows(q=q, cache_k=cache_k, cache_v=cache_v, tree_k=tree_k, tree_v=tree_v)
