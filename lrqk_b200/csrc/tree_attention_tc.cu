@@ -2,22 +2,27 @@
 // tree_plan.cuh.)
 //
 // A CTA walks its run of 128-key tiles with one or two blocks of 128 query rows (MT).  Per tile and row block
-//     S = Q K^T   tcgen05.mma M128 N128, K from a TMA tile (K-major), S in TMEM
-//     P = 2^(S c - m)   two threads per row, 64 keys each
-//     O += P V    tcgen05.mma with P read from TMEM and V from its TMA tile (N = head_dim, MN-major), O in TMEM; in two halves
-// One row block: S has two buffers, the scores run a tile ahead.  P enters the product as TWO bf16 parts, high and low, over
-// the columns of S that it replaces: one bf16 would add as much error as the final rounding of the result, and the extra
-// product hides behind the loads (per tile 1536 of the 2800 cycles that HBM needs).
-// Two row blocks: 512 columns of TMEM hold two O and one S buffer each, one block's products run while the other's
-// weights are formed, and P is ONE bf16: with two parts the products alone would take 3072 of those 2800 cycles.
+//     S = Q K^T   tcgen05.mma M128, K from a TMA tile (K-major), S in TMEM
+//     P = 2^(S c - m)   a thread per row, 64 keys at a time, in the place of their scores
+//     O += P V    tcgen05.mma with P read from TMEM and V from its TMA tile (N = head_dim, MN-major), O in TMEM, per 64 keys
+// One row block: S has two buffers, the scores run a tile ahead.  P enters the product as TWO bf16 parts, high and low: one
+// bf16 would add as much error as the final rounding of the result, and the extra product hides behind the loads (three
+// products of 512 cycles in the 2800 that HBM needs for a tile).
+// Two row blocks: 512 columns of TMEM hold two O and one S buffer each, and P is ONE bf16: six products would take longer
+// than the loads.  The scores of 64 keys are replaced by the next tile's as soon as their product with the values is
+// issued, so that four (row block, 64 keys) pipelines are under way; waiting for a tile's both halves cost as much as the
+// products of 64 columns lose.
 // The running maximum moves only when a row's maximum has grown by more than 2^8 (then O is read, scaled and written
 // back by the row's thread); weights then stay below 2^8 and sums keep fp32's full precision.
 //
 // Warp 0 issues the copies (a ring of K and V tiles, 128-byte swizzle), warp 1 owns TMEM and issues the products, warps
-// 2.. form the weights: a warp has 32 rows and one half of a tile's keys.  The maximum in use of a row passes from one half
-// to the next (of this tile, of the next one).  With two row blocks the second half does not wait for the first: it forms its
-// weights against the maximum it knows and looks afterwards whether the first half moved it, in which case it forms them
-// again (rarely); waiting ahead of the weights cost that kernel a fifth of its time.
+// 2.. form the weights, 32 rows a warp.  (Two threads per row, a half of the keys each, had to hand the maximum from one to
+// the other: 270 instead of 250 us for 64 nodes over two full contexts.)
+//
+// What bounds it: one row block runs at 150-165 us over two full contexts of 119156 rows (992 MB: 6.0-6.6 TB/s) up to 16
+// nodes.  With two row blocks the weights do: per tile and warp two times 64 keys of about 1400 cycles, 900 of them the
+// exponentials, which two warps of a scheduler share (2048 cycles a tile), against 2800 cycles of loads.  Exponentials by
+// polynomial for a quarter or half of the keys made it slower, as did forming them ahead of the maximum.
 //
 // V rows behind a length may hold anything, and 0 * NaN is NaN: the softmax warps clear them in shared memory before the
 // product.  In a drafted tile, values of V out of range are replaced by zeros and their nodes noted; a row that sees such
@@ -43,16 +48,14 @@ template <int D, int MT> struct Shape {
   static constexpr int kHalfBytes = kTileKeys * 128;                 // 64 columns of a tile
   static constexpr int kQBytes = MT * kBlockRows * D * 2;
   static constexpr int kStages = (208 * 1024 - kQBytes) / kTileBytes > 8 ? 8 : (208 * 1024 - kQBytes) / kTileBytes;
-  static constexpr int kThreads = 64 + 256 * MT;
+  static constexpr int kThreads = 64 + 128 * MT;
   static constexpr size_t kSmem = kQBytes + (size_t)kStages * kTileBytes + 1024;
 };
 
 struct Barriers {
   uint64_t full[8], empty[8], q_full;
-  // [S buffer (one row block) or row block (two)], and the half of the keys
-  uint64_t s_full[2], p_ready[2][2], o_done[2][2];
-  uint64_t decided[2][2][4], pair[2][4];    // [row block][half][32 rows]: the maximum in use is set; [row block][32 rows]
-  float top[2][kBlockRows], sum[2][2][kBlockRows];
+  // [S buffer (one row block) or row block (two)], and the half of the keys (scores of one row block: both in [0])
+  uint64_t s_full[2][2], p_ready[2][2], o_done[2][2];
   uint32_t tmem, give_up, odd[2][4];        // odd: drafted rows of V with values out of range, 128 bits for each drafted tile
   int32_t x0, x1, base, seq;
 };
@@ -253,11 +256,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) { mbar_init(&bar.full[i], 1); mbar_init(&bar.empty[i], 1); }
-    for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1);
-    for (int i = 0; i < 4; ++i) { mbar_init(&bar.p_ready[i >> 1][i & 1], 4); mbar_init(&bar.o_done[i >> 1][i & 1], 1); }
-    for (int i = 0; i < 16; ++i) mbar_init(&bar.decided[i >> 3][(i >> 2) & 1][i & 3], 1);
-    for (int i = 0; i < 8; ++i) mbar_init(&bar.pair[i >> 2][i & 3], 2);
-    mbar_init(&bar.q_full, 8 * MT);
+    for (int i = 0; i < 4; ++i) { mbar_init(&bar.s_full[i >> 1][i & 1], 1); mbar_init(&bar.p_ready[i >> 1][i & 1], 4); mbar_init(&bar.o_done[i >> 1][i & 1], 1); }
+    mbar_init(&bar.q_full, 4 * MT);
     bar.give_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -311,7 +311,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     }
   } else if (warp == 1) {
     // ---- products: the whole warp walks along, so that descriptors stay in uniform registers; one lane issues ----------------
-    constexpr uint32_t kIdescS = umma_idesc_bf16_k(128, kTileKeys);
+    constexpr int kScoreKeys = MT == 1 ? kTileKeys : kTileKeys / 2;            // keys of one scores product
+    constexpr uint32_t kIdescS = umma_idesc_bf16_k(128, kScoreKeys);
     constexpr uint32_t kIdescO = umma_idesc_bf16_k(128, D) | (1u << 16);       // B (the values) MN-major
     const uint32_t leader = elect_one();
     const uint64_t q_desc = umma_desc_k_sw128(saddr(qs), 1024), k_desc = umma_desc_k_sw128(saddr(stages), 1024);
@@ -321,37 +322,33 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       quit();
       return false;
     };
-    // (Addresses in descriptors count 16 bytes.)  `i`: ring index of the tile; x: its scores' buffer.
-    const auto scores = [&](int i, int m, int x) {
-      const uint64_t kd = k_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes) >> 4), qd = q_desc + (uint64_t)(m * ((kBlockRows * D * 2) >> 4));
+    // (Addresses in descriptors count 16 bytes.)  `i`: ring index of the tile; x: its scores' buffer; part: which kScoreKeys.
+    const auto scores = [&](int i, int m, int x, int part) {
+      const uint64_t kd = k_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes + part * kScoreKeys * 128) >> 4), qd = q_desc + (uint64_t)(m * ((kBlockRows * D * 2) >> 4));
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const uint64_t off = ((ks >> 2) * S::kHalfBytes + (ks & 3) * 32) >> 4;
-        umma_ss(tmem + x * 128, qd + off, kd + off, kIdescS, ks > 0, leader);
+        umma_ss(tmem + x * 128 + part * kScoreKeys, qd + off, kd + off, kIdescS, ks > 0, leader);
       }
-      commit(&bar.s_full[x], leader);
+      commit(&bar.s_full[x][part], leader);
     };
-    // the product with the values, each half of the keys as soon as its weights are there
-    const auto values = [&](int i, int m, int x, uint32_t parity, bool fresh) {
-      const uint32_t d = tmem + kOCol + m * 128;
+    // the product of one half of a tile's keys with the values, as soon as its weights are there
+    const auto values = [&](int i, int m, int x, int half, uint32_t parity, bool fresh) {
+      const uint32_t d = tmem + kOCol + m * 128, a = tmem + x * 128 + half * 64;
+      if (!ready(&bar.p_ready[x][half], parity)) return false;
+      const uint64_t vd = v_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes + half * 64 * 128) >> 4);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (!ready(&bar.p_ready[x][half], parity)) return false;
-        const uint64_t vd = v_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes + half * 64 * 128) >> 4);
-        const uint32_t a = tmem + x * 128 + half * 64;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const bool add = !(fresh && half == 0 && ks == 0);
-          if constexpr (MT == 1) {         // per 32 keys: 16 columns of high parts, 16 of low parts
-            const uint32_t at = a + (ks >> 1) * 32 + (ks & 1) * 8;
-            umma_ts(d, at, vd + ks * (2048 >> 4), kIdescO, add, leader);
-            umma_ts(d, at + 16, vd + ks * (2048 >> 4), kIdescO, 1, leader);
-          } else {
-            umma_ts(d, a + ks * 8, vd + ks * (2048 >> 4), kIdescO, add, leader);
-          }
+      for (int ks = 0; ks < 4; ++ks) {
+        const bool add = !(fresh && half == 0 && ks == 0);
+        if constexpr (MT == 1) {         // per 32 keys: 16 columns of high parts, 16 of low parts
+          const uint32_t at = a + (ks >> 1) * 32 + (ks & 1) * 8;
+          umma_ts(d, at, vd + ks * (2048 >> 4), kIdescO, add, leader);
+          umma_ts(d, at + 16, vd + ks * (2048 >> 4), kIdescO, 1, leader);
+        } else {
+          umma_ts(d, a + ks * 8, vd + ks * (2048 >> 4), kIdescO, add, leader);
         }
-        commit(&bar.o_done[x][half], leader);
       }
+      commit(&bar.o_done[x][half], leader);
       return true;
     };
     const auto arrived = [&](int i) { return ready(&bar.full[i % S::kStages], (i / S::kStages) & 1); };
@@ -362,36 +359,38 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       bool ok = ready(&bar.q_full, seg & 1) && arrived(i);
       if (!ok) break;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) scores(i, m, MT == 1 ? cnt & 1 : m);
+      for (int k = 0; k < (MT == 1 ? 1 : 4); ++k) scores(i, k >> 1, MT == 1 ? cnt & 1 : k >> 1, k & 1);
       release(i);
       for (int t = 0; t < n; ++t, ++cnt, i += 2) {
         const bool more = t + 1 < n;
         if constexpr (MT == 1) {
           if (more) {
             if (!(ok = arrived(i + 2))) break;
-            scores(i + 2, 0, (cnt + 1) & 1);
+            scores(i + 2, 0, (cnt + 1) & 1, 0);
             release(i + 2);
           }
-          if (!(ok = arrived(i + 1) && values(i + 1, 0, cnt & 1, (cnt >> 1) & 1, t == 0))) break;
+          const uint32_t parity = (cnt >> 1) & 1;
+          if (!(ok = arrived(i + 1) && values(i + 1, 0, cnt & 1, 0, parity, t == 0) && values(i + 1, 0, cnt & 1, 1, parity, t == 0))) break;
         } else {
-          if (!(ok = arrived(i + 1) && values(i + 1, 0, 0, cnt & 1, t == 0))) break;
-          if (more) {
-            if (!(ok = arrived(i + 2))) break;
-            scores(i + 2, 0, 0);
+          if (!(ok = arrived(i + 1))) break;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {    // (row block, half): the scores of the next tile replace weights that are used
+            if (!(ok = ok && values(i + 1, k >> 1, k >> 1, k & 1, cnt & 1, t == 0))) continue;
+            if (more) {
+              if (k == 0 && !(ok = arrived(i + 2))) continue;
+              scores(i + 2, k >> 1, k >> 1, k & 1);
+            }
           }
-          if (!(ok = values(i + 1, 1, 1, cnt & 1, t == 0))) break;
-          if (more) {
-            scores(i + 2, 1, 1);
-            release(i + 2);
-          }
+          if (!ok) break;
+          if (more) release(i + 2);
         }
         release(i + 1);
       }
       if (!ok) break;
     }
   } else {
-    // ---- weights: two threads per query row, 64 keys of a tile each ----------------------------------------------------------
-    const int m = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1;                             // row block, half of the keys
+    // ---- weights: a thread per query row -------------------------------------------------------------------------------------
+    const int m = (warp - 2) >> 2;                                                           // row block
     const int quarter = warp & 3, r_in = quarter * 32 + lane, row = m * kBlockRows + r_in;   // TMEM lanes 32 * (warp % 4)..
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), o_base = lane_base + kOCol + m * 128;
     const int g = group_row(p, row0 + row), node = row0 + row - g * p.nodes;                // query head in the group, node
@@ -403,11 +402,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     };
     for (; w.valid() && !*give_up; w.next(p), ++seg) {
       // the block's queries, for the K-major swizzled operand (rows that do not exist: zeros); all loads in flight at once
-      constexpr int kLoaders = 256, kLoads = kBlockRows * (D / 8) / kLoaders;
+      constexpr int kLoaders = 128, kLoads = kBlockRows * (D / 8) / kLoaders;
       uint4 qv[kLoads];
       {
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + w.b * p.q_stride[0] + (int64_t)(w.head * per_head) * p.q_stride[1];
-        const int first = half * 128 + quarter * 32 + lane;
+        const int first = quarter * 32 + lane;
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
           const int e = first + k * kLoaders, r = m * kBlockRows + e / (D / 8), c = e % (D / 8);
@@ -417,13 +416,13 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         }
       }
       // which nodes of a drafted step this row sees
-      uint32_t seen[2] = {0, 0};
+      uint32_t seen[4] = {0, 0, 0, 0};
       int seen_at = -1;
       const auto look = [&](int at) {                    // a row of the mask at a time, a lane per node: coalesced, no exchange
         seen_at = at;
         const uint8_t *mask = p.mask ? p.mask + w.b * p.mask_stride : nullptr;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 4; ++c) {
           const int first = at + c * 32, j = first + lane;
           seen[c] = 0;
           if (first >= p.nodes) continue;
@@ -441,10 +440,10 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           }
         }
       };
-      if (warp_real && w.t1 > w.ctiles) look(max(w.t0 - w.ctiles, 0) * kTileKeys + half * 64);   // ahead of its use
+      if (warp_real && w.t1 > w.ctiles) look(max(w.t0 - w.ctiles, 0) * kTileKeys);   // ahead of its use
       {
         unsigned char *dst = qs + m * (kBlockRows * D * 2);
-        const int first = half * 128 + quarter * 32 + lane;
+        const int first = quarter * 32 + lane;
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
           const int e = first + k * kLoaders, r = e / (D / 8), c = e % (D / 8);
@@ -458,19 +457,16 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       for (int st = 0; st < n_tiles; ++st, ++cnt) {
         const int x = MT == 1 ? cnt & 1 : m;
         const uint32_t parity = MT == 1 ? (cnt >> 1) & 1 : cnt & 1;
-        const uint32_t s_base = lane_base + x * 128 + half * 64;
         const bool masked = st >= plain;
         int n_keys = kTileKeys, dt = -1;                 // filled keys of the tile; drafted tile
         if (masked) {
           dt = w.t0 + st - w.ctiles;
           n_keys = min(kTileKeys, dt >= 0 ? p.nodes - dt * kTileKeys : w.len - (w.t0 + st) * kTileKeys);
-          if (warp_real && dt >= 0 && dt * kTileKeys + half * 64 != seen_at) look(dt * kTileKeys + half * 64);
+          if (warp_real && dt >= 0 && dt * kTileKeys != seen_at) look(dt * kTileKeys);
         }
         const bool drafted = dt >= 0;
-        if (!await(&bar.s_full[x], parity)) { quit(); break; }
-        fence_after();
         // values that must not meet the product: rows of the cache behind the length, drafted rows out of range
-        if (masked && m == 0 && half == 0) {
+        if (masked && m == 0) {
           const int i = i0 + 2 * st;
           const int vi = (i + 1) % S::kStages;
           unsigned char *vt = stages + (size_t)vi * S::kTileBytes;
@@ -510,94 +506,62 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        if (warp_real) {
-          uint32_t v[32], u[32];
-          load32_async(s_base, v);
-          load32_async(s_base + 32, u);
-          load_wait();
-          pin(v);
-          pin(u);
-          if (masked) {
-            const int n = n_keys - half * 64;            // filled keys of this half
-            hide(v, drafted ? seen[0] : n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u);
-            hide(u, drafted ? seen[1] : n >= 64 ? 0xFFFFFFFFu : n > 32 ? (1u << (n - 32)) - 1u : 0u);
-          }
-          const float now = fmaxf(max32(v), max32(u)) * p.scale_log2;
-          const float old = top;
-          const auto grown = [&](float in_use) { return now > in_use + kGrow || (in_use == -INFINITY && now > -INFINITY); };
-          // the second half of two row blocks goes ahead unless it would move the maximum itself, or knows none yet.  (With one
-          // row block the first half may be a tile ahead and move the maximum again before this one has looked.)
-          const bool ahead = MT == 2 && half == 1 && st > 0 && !__any_sync(0xFFFFFFFFu, grown(top));
-          if (ahead) {
-            signal(&bar.decided[m][1][quarter]);
-          } else {
-            // the maximum in use, from the half before (with two row blocks the scores of a tile follow its products: known)
-            if (half == 1 || (MT == 1 && cnt > 0)) {
-              if (!await(&bar.decided[m][half ^ 1][quarter], (half == 1 ? cnt : cnt - 1) & 1)) { quit(); break; }
+        bool ok = true;
+#pragma unroll
+        for (int half = 0; half < 2 && ok; ++half) {
+          if ((MT == 2 || half == 0) && !(ok = await(&bar.s_full[x][half], parity))) break;
+          fence_after();
+          const uint32_t s_base = lane_base + x * 128 + half * 64;
+          if (warp_real) {
+            uint32_t v[32], u[32];
+            load32_async(s_base, v);
+            load32_async(s_base + 32, u);
+            load_wait();
+            pin(v);
+            pin(u);
+            if (masked) {
+              const int n = n_keys - half * 64;          // filled keys of this half
+              hide(v, drafted ? seen[2 * half] : n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u);
+              hide(u, drafted ? seen[2 * half + 1] : n >= 64 ? 0xFFFFFFFFu : n > 32 ? (1u << (n - 32)) - 1u : 0u);
             }
-            if (half == 1 || st > 0) top = bar.top[m][r_in];
-            const bool move = grown(top);
-            const float use = move ? now : top;
-            if (move || (half == 0 && st == 0)) bar.top[m][r_in] = use;
-            signal(&bar.decided[m][half][quarter]);
-            if (__any_sync(0xFFFFFFFFu, move) && (half == 1 || st > 0)) {
-              // O holds the products up to the half before: that one has to be in it
-              const int px = MT == 1 ? (half == 1 ? x : x ^ 1) : m, pc = half == 1 ? cnt : cnt - 1;
-              if (!await(&bar.o_done[px][half ^ 1], (MT == 1 ? pc >> 1 : pc) & 1)) { quit(); break; }
-              fence_after();
-              const float fade = move ? exp2_fast(top - use) : 1.0f;
+            const float now = fmaxf(max32(v), max32(u)) * p.scale_log2;
+            const bool move = now > top + kGrow || (top == -INFINITY && now > -INFINITY);
+            if (__any_sync(0xFFFFFFFFu, move)) {
+              const float use = move ? now : top, fade = move ? exp2_fast(top - use) : 1.0f;
+              if (half == 1 || st > 0) {
+                // O holds the products up to the half before: that one has to be in it
+                const int px = MT == 1 ? (half == 1 ? x : x ^ 1) : m, pc = half == 1 ? cnt : cnt - 1;
+                if (!(ok = await(&bar.o_done[px][half ^ 1], (MT == 1 ? pc >> 1 : pc) & 1))) break;
+                fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D; c += 8) scale8(o_base + c, fade);
+                for (int c = 0; c < D; c += 8) scale8(o_base + c, fade);
+              }
+              sum *= fade;
+              top = use;
             }
-            top = use;
-          }
-          if (old != top) sum *= exp2_fast(old - top);
-          const uint64_t c2 = pair(p.scale_log2, p.scale_log2);
-          uint64_t sum2 = 0;
-          {
-            const uint64_t minus2 = top == -INFINITY ? 0 : pair(-top, -top);
+            const uint64_t c2 = pair(p.scale_log2, p.scale_log2), minus2 = top == -INFINITY ? 0 : pair(-top, -top);
+            uint64_t sum2 = 0;
             weigh(v, c2, minus2, sum2);
             weigh(u, c2, minus2, sum2);
-          }
-          if (ahead) {
-            if (!await(&bar.decided[m][0][quarter], cnt & 1)) { quit(); break; }
-            const float first = bar.top[m][r_in];
-            if (__any_sync(0xFFFFFFFFu, first != top)) {  // the first half moved it: again, from the scores in TMEM
-              if (first != top) sum *= exp2_fast(top - first);
-              top = first;
-              load32_async(s_base, v);
-              load32_async(s_base + 32, u);
-              load_wait();
-              pin(v);
-              pin(u);
-              if (masked) {
-                const int n = n_keys - half * 64;
-                hide(v, drafted ? seen[0] : n >= 32 ? 0xFFFFFFFFu : n > 0 ? (1u << n) - 1u : 0u);
-                hide(u, drafted ? seen[1] : n >= 64 ? 0xFFFFFFFFu : n > 32 ? (1u << (n - 32)) - 1u : 0u);
-              }
-              const uint64_t minus2 = top == -INFINITY ? 0 : pair(-top, -top);
-              sum2 = 0;
-              weigh(v, c2, minus2, sum2);
-              weigh(u, c2, minus2, sum2);
-            }
-          }
-          if constexpr (MT == 1) {
-            store_two_parts(v, s_base);
-            store_two_parts(u, s_base + 32);
-          } else {
-            uint32_t o[32];
+            if constexpr (MT == 1) {
+              store_two_parts(v, s_base);
+              store_two_parts(u, s_base + 32);
+            } else {
+              uint32_t o[32];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              o[j] = pack_bf16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-              o[16 + j] = pack_bf16(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+              for (int j = 0; j < 16; ++j) {
+                o[j] = pack_bf16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                o[16 + j] = pack_bf16(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+              }
+              store32(s_base, o);
             }
-            store32(s_base, o);
+            sum += low_of(sum2) + high_of(sum2);
           }
-          sum += low_of(sum2) + high_of(sum2);
+          store_wait();
+          fence_before();
+          signal(&bar.p_ready[x][half]);
         }
-        store_wait();
-        fence_before();
-        signal(&bar.p_ready[x][half]);
+        if (!ok) { quit(); break; }
       }
       i0 += 2 * n_tiles;
       if (*give_up) break;
@@ -606,19 +570,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         if (!await(&bar.o_done[x][1], (MT == 1 ? (cnt - 1) >> 1 : cnt - 1) & 1)) { quit(); break; }
         fence_after();
       }
-      // ---- the segment's rows: finished, or a partial; a row's threads share its columns ------------------------------------
+      // ---- the segment's rows: finished, or a partial -------------------------------------------------------------------------
       if (warp_real) {
-        if (half == 0) {                                 // the maximum that the last half set
-          if (!await(&bar.decided[m][1][quarter], (cnt - 1) & 1)) { quit(); break; }
-          const float last = bar.top[m][r_in];
-          if (last != top) sum *= exp2_fast(top - last);
-          top = last;
-        }
-        bar.sum[m][half][r_in] = sum;
-        signal(&bar.pair[m][quarter]);
-        if (!await(&bar.pair[m][quarter], seg & 1)) { quit(); break; }
-        sum += bar.sum[m][half ^ 1][r_in];
-        constexpr int kCols = D / 2;
         const bool whole = w.whole();
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int64_t at = ((int64_t)w.b * p.q_heads + w.head * per_head + g) * p.nodes + node;
@@ -627,8 +580,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         if (w.t1 > w.ctiles)
           for (int c = 0; c < 8; ++c) any_odd |= *reinterpret_cast<volatile uint32_t *>(&bar.odd[c >> 2][c & 3]);
 #pragma unroll
-        for (int cc = 0; cc < kCols; cc += 32) {
-          const int c = half * kCols + cc;
+        for (int c = 0; c < D; c += 32) {
           uint32_t v[32];
           load32(o_base + c, v);
           if (any_odd && real) {
@@ -661,7 +613,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             }
           }
         }
-        if (real && half == 0) {
+        if (real) {
           if (!whole) p.part_ml[slot] = make_float2(top, sum);
           else if (p.lse) p.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
         }
