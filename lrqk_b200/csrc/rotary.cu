@@ -13,6 +13,8 @@
 // Bound: HBM.  q and k are read once and written once; the angles come from registers, not from cos/sin tables.  A
 // thread owns one 16-byte run of pairs of one token, computes its cosines and sines once and applies them to a run
 // of heads, four heads' loads in flight at a time; with few tokens the heads are dealt over more threads instead.
+// Measured: 65536 tokens of 32 + 8 bf16 heads of 128, 1.34 GB in 219 us (6.1 TB/s, 94 % of a copy); one token of four
+// sequences 2.4 us; the adjoint of 2 x 1537 tokens of 28 + 4 fp32 heads 14.9 us (its 101 MB partly from L2).
 #include "common.cuh"
 
 namespace lrqk {

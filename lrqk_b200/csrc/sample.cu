@@ -20,7 +20,9 @@
 // sums of contiguous chunks and a second look at one chunk.
 //
 // Bound: the latency of the cluster barriers for few rows (each merge is two of them, 2.7 us with the reads between);
-// instructions -- the double exponential, three atomics a token -- for many.
+// barriers and instructions -- the double exponential, three atomics a token -- for many.  One row of 128256 bf16 logits
+// with top-k 50 takes 14 us, 25 rows with top-p alone 52 us, 64 rows of 152064 fp32 logits with mixed settings 71 us (39 MB:
+// 6 us of loads).
 #include <cooperative_groups.h>
 
 #include "common.cuh"

@@ -17,10 +17,11 @@
 //
 // Warp 0 issues the copies (a ring of K and V tiles, 128-byte swizzle), warp 1 owns TMEM and issues the products, warps
 // 2.. form the weights, 32 rows a warp.  (Two threads per row, a half of the keys each, had to hand the maximum from one to
-// the other: 270 instead of 250 us for 64 nodes over two full contexts.)
+// the other: 269 instead of 255 us for 64 nodes, and the two-block kernel spilled.)
 //
-// What bounds it: one row block runs at 150-165 us over two full contexts of 119156 rows (992 MB: 6.0-6.6 TB/s) up to 16
-// nodes.  With two row blocks the weights do: per tile and warp two times 64 keys of about 1400 cycles, 900 of them the
+// What bounds it, over two full contexts of 119156 rows and 8 cache heads (979 MB, 149.5 us at 6.55 TB/s), 4 query heads a
+// cache head: one row block takes 163 us with 1 node, 169 with 8, 180 with 16 and 200 with 32 (two threads per row: 157 to
+// 188, at the price of a second arrangement).  64 nodes, two row blocks: 255 us, and the weights bound it: per tile and warp two times 64 keys of about 1400 cycles, 900 of them the
 // exponentials, which two warps of a scheduler share (2048 cycles a tile), against 2800 cycles of loads.  Exponentials by
 // polynomial for a quarter or half of the keys made it slower, as did forming them ahead of the maximum.
 //
