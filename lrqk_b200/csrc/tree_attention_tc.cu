@@ -468,6 +468,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         const bool drafted = dt >= 0;
         // values that must not meet the product: rows of the cache behind the length, drafted rows out of range
         if (masked && m == 0) {
+          // (the scores are there once every warp has left the segment before, whose marks in `odd` these replace)
+          if (!await(&bar.s_full[x][0], parity)) { quit(); break; }
           const int i = i0 + 2 * st;
           const int vi = (i + 1) % S::kStages;
           unsigned char *vt = stages + (size_t)vi * S::kTileBytes;

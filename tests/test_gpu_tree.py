@@ -262,3 +262,21 @@ def test_refusals():
     grad = q.float().requires_grad_()
     with pytest.raises(ValueError):
         tree_attention(grad, ck.float(), cv.float(), tk.float(), tv.float())
+
+
+@pytest.mark.parametrize("t,spoilt", [(64, 63), (30, 29), (160, 130)])
+def test_values_out_of_range_in_some_of_many_short_sequences(t, spoilt):
+    """A CTA meets many (sequence, head) units in a row, each with other drafted values out of range: every row that sees one has
+    it, no other row has any."""
+    q, ck, cv, tk, tv = make(60, 32, 8, 8, t, 40, 128, torch.bfloat16, seed=5)[:5]
+    columns = [(7 * i + 3) % 128 for i in range(60)]
+    for i in range(0, 60, 2):
+        tv[i, :, spoilt, columns[i]] = math.inf
+    for lens in (torch.zeros(60, dtype=torch.int32, device="cuda"), torch.arange(60, dtype=torch.int32, device="cuda") % 41):
+        for _ in range(10):
+            out = tree_attention(q, ck, cv, tk, tv, cache_lens=lens)
+            want = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+            for i in range(0, 60, 2):
+                want[i, :, spoilt:, columns[i]] = True
+            assert torch.equal(torch.isinf(out), want) and not bool(torch.isnan(out).any())
+    check_tree_status()
