@@ -1005,10 +1005,10 @@ class DynamicLRQKCache(_CacheBase):
         t = next(iter(self._drafted.values()))[0].shape[2]
         if any(not 0 <= i < t for i in nodes) or any(b <= a for a, b in zip(nodes, nodes[1:])):
             raise ValueError(f"nodes {nodes}: ascending indices below {t} are expected")
-        for layer_idx, (q, k, v) in self._drafted.items():
+        drafted, self._drafted = self._drafted, {}               # an error half-way leaves nothing to decode twice
+        for layer_idx, (q, k, v) in drafted.items():
             for i in nodes:
                 self.lwattn[layer_idx]._decode(q[:, :, i:i + 1], k[:, :, i:i + 1], v[:, :, i:i + 1], attention=False)
-        self._drafted = {}
 
     def state_dict(self) -> dict:
         """The whole cache for ``load_state_dict``: every decoding layer's ``state_dict()`` and the prompt rows of

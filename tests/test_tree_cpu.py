@@ -41,3 +41,29 @@ def test_workspace_of_refused_shapes_is_zero():
                 dict(head_dim=96), dict(capacity=-1), dict(capacity=1 << 31), dict(q_heads=1 << 16, cache_heads=1, tree_heads=1, nodes=256)):
         assert ws(**bad) == 0, bad
     assert lib.lrqk_tree_attention_workspace_bytes(None) == 0
+
+
+def test_an_error_while_accepting_leaves_nothing_to_decode_twice():
+    from lrqk_b200 import DynamicLRQKCache
+
+    class Layer:
+        def __init__(self, fails):
+            self.fails, self.steps = fails, 0
+
+        def _decode(self, q, k, v, attention):
+            if self.fails:
+                raise RuntimeError("full")
+            self.steps += 1
+
+        def close(self):
+            pass
+
+    cache = DynamicLRQKCache(r=8, num_active_tokens=16, lite_tokens=4, num_key_value_groups=1)
+    cache.lwattn = {0: Layer(False), 1: Layer(True)}
+    row = torch.zeros(1, 1, 3, 64)
+    cache._drafted = {0: (row, row, row), 1: (row, row, row)}
+    with pytest.raises(RuntimeError, match="full"):
+        cache.accept([0, 2])
+    with pytest.raises(RuntimeError, match="no drafted"):
+        cache.accept([0, 2])
+    assert cache.lwattn[0].steps == 2
