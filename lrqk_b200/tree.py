@@ -49,7 +49,7 @@ def _status_word(device: torch.device) -> Optional[int]:
             return None
         word = torch.zeros(4, dtype=torch.int32, device=device)
         torch.cuda.current_stream(device).synchronize()
-        _status[device.index] = word
+        word = _status.setdefault(device.index, word)            # (two threads' first calls: one word)
     return word.data_ptr()
 
 
