@@ -5,9 +5,11 @@
 //     S = Q K^T   tcgen05.mma M128, K from a TMA tile (K-major), S in TMEM
 //     P = 2^(S c - m)   a thread per row, 64 keys at a time, in the place of their scores
 //     O += P V    tcgen05.mma with P read from TMEM and V from its TMA tile (N = head_dim, MN-major), O in TMEM, per 64 keys
-// One row block: S has two buffers, the scores run a tile ahead.  P enters the product as TWO bf16 parts, high and low: one
-// bf16 would add as much error as the final rounding of the result, and the extra product hides behind the loads (three
-// products of 512 cycles in the 2800 that HBM needs for a tile).
+// Two chains of softmax warps work side by side, each with an S buffer, an O, a maximum and a sum of its own: with one row
+// block on alternate tiles of the same rows (joined at a segment's end), with two on a block each.
+// One row block: the scores run a tile ahead.  P enters the product as TWO bf16 parts, high and low: one bf16 would add
+// as much error as the final rounding of the result, and the extra product hides behind the loads (three products of 512
+// cycles in the 2800 that HBM needs for a tile).
 // Two row blocks: 512 columns of TMEM hold two O and one S buffer each, and P is ONE bf16: six products would take longer
 // than the loads.  The scores of 64 keys are replaced by the next tile's as soon as their product with the values is
 // issued, so that four (row block, 64 keys) pipelines are under way; waiting for a tile's both halves cost as much as the
@@ -16,14 +18,16 @@
 // back by the row's thread); weights then stay below 2^8 and sums keep fp32's full precision.
 //
 // Warp 0 issues the copies (a ring of K and V tiles, 128-byte swizzle), warp 1 owns TMEM and issues the products, warps
-// 2.. form the weights, 32 rows a warp.  (Two threads per row, a half of the keys each, had to hand the maximum from one to
-// the other: 269 instead of 255 us for 64 nodes, and the two-block kernel spilled.)
+// 2..9 form the weights, 32 rows a warp.  (Two threads per row, a half of each tile's keys each, had to hand the maximum from
+// one to the other: 269 instead of 253 us for 64 nodes, 190 instead of 187 for 32, and the two-block kernel spilled.  One chain for
+// one row block: 163 instead of 159 us with 1 node, 200 instead of 187 with 32.)
 //
 // What bounds it, over two full contexts of 119156 rows and 8 cache heads (979 MB, 149.5 us at 6.55 TB/s), 4 query heads a
-// cache head: one row block takes 163 us with 1 node, 169 with 8, 180 with 16 and 200 with 32 (two threads per row: 157 to
-// 188, at the price of a second arrangement).  64 nodes, two row blocks: 255 us, and the weights bound it: per tile and warp two times 64 keys of about 1400 cycles, 900 of them the
-// exponentials, which two warps of a scheduler share (2048 cycles a tile), against 2800 cycles of loads.  Exponentials by
-// polynomial for a quarter or half of the keys made it slower, as did forming them ahead of the maximum.
+// cache head: one row block takes 159 us with 1 node, 163 with 8, 171 with 16 and 187 with 32: HBM, and with more rows the
+// products and exponentials beside it.  64 nodes, two row blocks: 253 us, and the weights bound it: per tile and warp two times
+// 64 keys of about 1400 cycles, 900 of them the exponentials, which two warps of a scheduler share (2048 cycles a tile),
+// against 2800 cycles of loads.  Exponentials by polynomial for a quarter or half of the keys made it slower, as did forming
+// them ahead of the maximum.
 //
 // V rows behind a length may hold anything, and 0 * NaN is NaN: the softmax warps clear them in shared memory before the
 // product.  In a drafted tile, values of V out of range are replaced by zeros and their nodes noted; a row that sees such
@@ -42,21 +46,23 @@ using namespace tc;
 
 constexpr int kTileKeys = 128, kBlockRows = 128;
 constexpr float kGrow = 8.0f;     // octaves a maximum may grow before O is rescaled
-constexpr int kOCol = 256;        // TMEM columns: S 0..255, O 256 + 128 * row block
+constexpr int kOCol = 256;        // TMEM columns: S 0..255, O 256 + 128 * chain
 
 template <int D, int MT> struct Shape {
   static constexpr int kTileBytes = kTileKeys * D * 2;
   static constexpr int kHalfBytes = kTileKeys * 128;                 // 64 columns of a tile
   static constexpr int kQBytes = MT * kBlockRows * D * 2;
   static constexpr int kStages = (208 * 1024 - kQBytes) / kTileBytes > 8 ? 8 : (208 * 1024 - kQBytes) / kTileBytes;
-  static constexpr int kThreads = 64 + 128 * MT;
+  static constexpr int kThreads = 64 + 256;
   static constexpr size_t kSmem = kQBytes + (size_t)kStages * kTileBytes + 1024;
 };
 
 struct Barriers {
   uint64_t full[8], empty[8], q_full;
-  // [S buffer (one row block) or row block (two)], and the half of the keys (scores of one row block: both in [0])
+  // [chain], and the half of the keys (scores of one row block: both in [0])
   uint64_t s_full[2][2], p_ready[2][2], o_done[2][2];
+  uint64_t joined[4];                       // one row block: both chains' maximum and sum of 32 rows are in `ml`
+  float2 ml[2][kBlockRows];
   uint32_t tmem, give_up, odd[2][4];        // odd: drafted rows of V with values out of range, 128 bits for each drafted tile
   int32_t x0, x1, base, seq;
 };
@@ -258,7 +264,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) { mbar_init(&bar.full[i], 1); mbar_init(&bar.empty[i], 1); }
     for (int i = 0; i < 4; ++i) { mbar_init(&bar.s_full[i >> 1][i & 1], 1); mbar_init(&bar.p_ready[i >> 1][i & 1], 4); mbar_init(&bar.o_done[i >> 1][i & 1], 1); }
-    mbar_init(&bar.q_full, 4 * MT);
+    for (int i = 0; i < 4; ++i) mbar_init(&bar.joined[i], 2);
+    mbar_init(&bar.q_full, 8);
     bar.give_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -334,8 +341,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       commit(&bar.s_full[x][part], leader);
     };
     // the product of one half of a tile's keys with the values, as soon as its weights are there
-    const auto values = [&](int i, int m, int x, int half, uint32_t parity, bool fresh) {
-      const uint32_t d = tmem + kOCol + m * 128, a = tmem + x * 128 + half * 64;
+    const auto values = [&](int i, int x, int half, uint32_t parity, bool fresh) {
+      const uint32_t d = tmem + kOCol + x * 128, a = tmem + x * 128 + half * 64;
       if (!ready(&bar.p_ready[x][half], parity)) return false;
       const uint64_t vd = v_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes + half * 64 * 128) >> 4);
 #pragma unroll
@@ -371,12 +378,12 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             release(i + 2);
           }
           const uint32_t parity = (cnt >> 1) & 1;
-          if (!(ok = arrived(i + 1) && values(i + 1, 0, cnt & 1, 0, parity, t == 0) && values(i + 1, 0, cnt & 1, 1, parity, t == 0))) break;
+          if (!(ok = arrived(i + 1) && values(i + 1, cnt & 1, 0, parity, t < 2) && values(i + 1, cnt & 1, 1, parity, t < 2))) break;
         } else {
           if (!(ok = arrived(i + 1))) break;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {    // (row block, half): the scores of the next tile replace weights that are used
-            if (!(ok = ok && values(i + 1, k >> 1, k >> 1, k & 1, cnt & 1, t == 0))) continue;
+            if (!(ok = ok && values(i + 1, k >> 1, k & 1, cnt & 1, t == 0))) continue;
             if (more) {
               if (k == 0 && !(ok = arrived(i + 2))) continue;
               scores(i + 2, k >> 1, k >> 1, k & 1);
@@ -391,9 +398,9 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     }
   } else {
     // ---- weights: a thread per query row -------------------------------------------------------------------------------------
-    const int m = (warp - 2) >> 2;                                                           // row block
+    const int chain = (warp - 2) >> 2, m = MT == 1 ? 0 : chain;                              // row block
     const int quarter = warp & 3, r_in = quarter * 32 + lane, row = m * kBlockRows + r_in;   // TMEM lanes 32 * (warp % 4)..
-    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), o_base = lane_base + kOCol + m * 128;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), o_base = lane_base + kOCol + chain * 128;
     const int g = group_row(p, row0 + row), node = row0 + row - g * p.nodes;                // query head in the group, node
     const bool real = row < n_rows, warp_real = m * kBlockRows + quarter * 32 < n_rows;
     int cnt = 0, i0 = 0, seg = 0;                        // tiles done, ring index of the segment's first K, segments done
@@ -403,11 +410,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     };
     for (; w.valid() && !*give_up; w.next(p), ++seg) {
       // the block's queries, for the K-major swizzled operand (rows that do not exist: zeros); all loads in flight at once
-      constexpr int kLoaders = 128, kLoads = kBlockRows * (D / 8) / kLoaders;
+      constexpr int kLoaders = MT == 1 ? 256 : 128, kLoads = kBlockRows * (D / 8) / kLoaders;
       uint4 qv[kLoads];
       {
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + w.b * p.q_stride[0] + (int64_t)(w.head * per_head) * p.q_stride[1];
-        const int first = quarter * 32 + lane;
+        const int first = (MT == 1 ? chain * 128 : 0) + quarter * 32 + lane;
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
           const int e = first + k * kLoaders, r = m * kBlockRows + e / (D / 8), c = e % (D / 8);
@@ -444,7 +451,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       if (warp_real && w.t1 > w.ctiles) look(max(w.t0 - w.ctiles, 0) * kTileKeys);   // ahead of its use
       {
         unsigned char *dst = qs + m * (kBlockRows * D * 2);
-        const int first = quarter * 32 + lane;
+        const int first = (MT == 1 ? chain * 128 : 0) + quarter * 32 + lane;
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
           const int e = first + k * kLoaders, r = e / (D / 8), c = e % (D / 8);
@@ -456,7 +463,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       float top = -INFINITY, sum = 0.0f;                 // maximum in use, in octaves; sum of this thread's weights
       const int n_tiles = w.t1 - w.t0, plain = w.len / kTileKeys - w.t0;   // the first `plain` tiles are seen whole
       for (int st = 0; st < n_tiles; ++st, ++cnt) {
-        const int x = MT == 1 ? cnt & 1 : m;
+        if (MT == 1 && (cnt & 1) != chain) continue;     // the other chain's tile
+        const int x = chain;
         const uint32_t parity = MT == 1 ? (cnt >> 1) & 1 : cnt & 1;
         const bool masked = st >= plain;
         int n_keys = kTileKeys, dt = -1;                 // filled keys of the tile; drafted tile
@@ -531,10 +539,9 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             const bool move = now > top + kGrow || (top == -INFINITY && now > -INFINITY);
             if (__any_sync(0xFFFFFFFFu, move)) {
               const float use = move ? now : top, fade = move ? exp2_fast(top - use) : 1.0f;
-              if (half == 1 || st > 0) {
-                // O holds the products up to the half before: that one has to be in it
-                const int px = MT == 1 ? (half == 1 ? x : x ^ 1) : m, pc = half == 1 ? cnt : cnt - 1;
-                if (!(ok = await(&bar.o_done[px][half ^ 1], (MT == 1 ? pc >> 1 : pc) & 1))) break;
+              if (half == 1 || st >= (MT == 1 ? 2 : 1)) {
+                // O holds the chain's products up to the half before: that one has to be in it
+                if (!(ok = await(&bar.o_done[x][half ^ 1], half == 1 ? parity : parity ^ 1))) break;
                 fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D; c += 8) scale8(o_base + c, fade);
@@ -568,13 +575,34 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       }
       i0 += 2 * n_tiles;
       if (*give_up) break;
-      {
-        const int x = MT == 1 ? (cnt - 1) & 1 : m;
-        if (!await(&bar.o_done[x][1], (MT == 1 ? (cnt - 1) >> 1 : cnt - 1) & 1)) { quit(); break; }
+      // (a segment of one tile leaves the chain that had none without an O)
+      const bool last_mine = MT == 2 || ((cnt - 1) & 1) == chain, mine = last_mine || n_tiles > 1;
+      if (mine) {
+        const int last = last_mine ? cnt - 1 : cnt - 2;
+        if (!await(&bar.o_done[chain][1], (MT == 1 ? last >> 1 : last) & 1)) { quit(); break; }
+        fence_after();
+      }
+      if constexpr (MT == 1) {                           // each chain's O and statistics for the other's warp of the same rows
+        bar.ml[chain][r_in] = make_float2(top, sum);
+        fence_before();
+        signal(&bar.joined[quarter]);
+        if (!await(&bar.joined[quarter], seg & 1)) { quit(); break; }
         fence_after();
       }
       // ---- the segment's rows: finished, or a partial -------------------------------------------------------------------------
       if (warp_real) {
+        float fade = 1.0f, other_fade = 0.0f;            // one row block: factors on the two chains' O
+        if constexpr (MT == 1) {
+          const float2 other = bar.ml[chain ^ 1][r_in];
+          const float both = fmaxf(top, other.x);
+          fade = top == both ? 1.0f : exp2_fast(top - both);
+          other_fade = other.x == both ? 1.0f : exp2_fast(other.x - both);
+          sum = sum * fade + other.y * other_fade;
+          top = both;
+        }
+        const bool others = MT == 1 && (n_tiles > 1 || !mine);
+        constexpr int kCols = MT == 1 ? D / 2 : D;       // columns of a thread: a row's two chains share them
+        const int c0 = MT == 1 ? chain * kCols : 0;
         const bool whole = w.whole();
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int64_t at = ((int64_t)w.b * p.q_heads + w.head * per_head + g) * p.nodes + node;
@@ -583,9 +611,17 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         if (w.t1 > w.ctiles)
           for (int c = 0; c < 8; ++c) any_odd |= *reinterpret_cast<volatile uint32_t *>(&bar.odd[c >> 2][c & 3]);
 #pragma unroll
-        for (int c = 0; c < D; c += 32) {
+        for (int cc = 0; cc < kCols; cc += 32) {
+          const int c = c0 + cc;
           uint32_t v[32];
-          load32(o_base + c, v);
+          if (mine) load32(o_base + c, v);
+          if constexpr (MT == 1) {
+            uint32_t u[32];
+            if (others) load32(lane_base + kOCol + (chain ^ 1) * 128 + c, u);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              v[e] = __float_as_uint((mine ? __uint_as_float(v[e]) * fade : 0.0f) + (others ? __uint_as_float(u[e]) * other_fade : 0.0f));
+          }
           if (any_odd && real) {
             // values out of range of the nodes this row sees, in the tiles of this segment
             for (int dt = max(w.t0 - w.ctiles, 0); dt < w.t1 - w.ctiles; ++dt)
@@ -616,7 +652,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             }
           }
         }
-        if (real) {
+        if (real && (MT == 2 || chain == 0)) {
           if (!whole) p.part_ml[slot] = make_float2(top, sum);
           else if (p.lse) p.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
         }
