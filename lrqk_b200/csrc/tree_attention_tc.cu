@@ -62,7 +62,10 @@ struct Barriers {
   // [chain], and the half of the keys (scores of one row block: both in [0])
   uint64_t s_full[2][2], p_ready[2][2], o_done[2][2];
   uint64_t joined[4];                       // one row block: both chains' maximum and sum of 32 rows are in `ml`
-  float2 ml[2][kBlockRows];
+  // ... [segment's parity][chain][row].  One buffer a parity: a warp whose chain has no tile of the next segment waits for
+  // nothing before it writes that segment's, while its partner may still be about to read this one's; two segments on,
+  // the `joined` between them has passed, which the partner signals behind its read.
+  float2 ml[2][2][kBlockRows];
   uint32_t tmem, give_up, odd[2][4];        // odd: drafted rows of V with values out of range, 128 bits for each drafted tile
   int32_t x0, x1, base, seq;
 };
@@ -583,7 +586,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         fence_after();
       }
       if constexpr (MT == 1) {                           // each chain's O and statistics for the other's warp of the same rows
-        bar.ml[chain][r_in] = make_float2(top, sum);
+        bar.ml[seg & 1][chain][r_in] = make_float2(top, sum);
         fence_before();
         signal(&bar.joined[quarter]);
         if (!await(&bar.joined[quarter], seg & 1)) { quit(); break; }
@@ -593,7 +596,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       if (warp_real) {
         float fade = 1.0f, other_fade = 0.0f;            // one row block: factors on the two chains' O
         if constexpr (MT == 1) {
-          const float2 other = bar.ml[chain ^ 1][r_in];
+          const float2 other = bar.ml[seg & 1][chain ^ 1][r_in];
           const float both = fmaxf(top, other.x);
           fade = top == both ? 1.0f : exp2_fast(top - both);
           other_fade = other.x == both ? 1.0f : exp2_fast(other.x - both);
