@@ -338,7 +338,7 @@ int plan(const lrqk_tree_args *a, Params &p) {
   if ((int64_t)a->q_heads / a->cache_heads * a->nodes > 1 << 16) return LRQK_EUNSUPPORTED;
   // The row blocks of a unit walk the same keys at the same time, so those come from HBM once.
   if (a->dtype == LRQK_BF16) {
-    if (!plan_tc(p)) return LRQK_EUNSUPPORTED;
+    plan_tc(p);
   } else {
     p.rows_per_block = kRows;
     p.tile_keys = kKeys;

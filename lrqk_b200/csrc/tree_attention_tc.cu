@@ -1,33 +1,33 @@
 // Tree attention on the tensor cores: bf16, head_dim 64 or 128.  (Formula, split and partials: tree_attention.cu,
 // tree_plan.cuh.)
 //
-// A CTA walks its run of 128-key tiles with one or two blocks of 128 query rows (MT).  Per tile and row block
+// A CTA walks its run of 128-key tiles with one block of 128 query rows.  Per tile
 //     S = Q K^T   tcgen05.mma M128, K from a TMA tile (K-major), S in TMEM
 //     P = 2^(S c - m)   a thread per row, 64 keys at a time, in the place of their scores
 //     O += P V    tcgen05.mma with P read from TMEM and V from its TMA tile (N = head_dim, MN-major), O in TMEM, per 64 keys
-// Two chains of softmax warps work side by side, each with an S buffer, an O, a maximum and a sum of its own: with one row
-// block on alternate tiles of the same rows (joined at a segment's end), with two on a block each.
-// One row block: the scores run a tile ahead.  P enters the product as TWO bf16 parts, high and low: one bf16 would add
-// as much error as the final rounding of the result, and the extra product hides behind the loads (three products of 512
-// cycles in the 2800 that HBM needs for a tile).
-// Two row blocks: 512 columns of TMEM hold two O and one S buffer each, and P is ONE bf16: six products would take longer
-// than the loads.  The scores of 64 keys are replaced by the next tile's as soon as their product with the values is
-// issued, so that four (row block, 64 keys) pipelines are under way; waiting for a tile's both halves cost as much as the
-// products of 64 columns lose.
+// Two chains of softmax warps work side by side on alternate tiles of the same rows, each with an S buffer, an O, a maximum and
+// a sum of its own, joined at a segment's end; the scores run a tile ahead.  P enters the product as TWO bf16 parts, high and
+// low: one bf16 would add as much error as the final rounding of the result, and under one row block the extra product hides
+// behind the loads (three products of 512 cycles in the 2800 that HBM needs for a tile).
+// More rows than a block: the blocks' CTAs walk the same tiles at the same time, each loading them for itself, so that HBM
+// reads them once and L2 hands them out.  (One CTA with two blocks and P as one bf16 took 254 us where this takes 318, for 64
+// nodes over two full contexts; but then a row lost accuracy, half a step of bf16 in each weight, as soon as other nodes made
+// the call larger.  The same with P in two parts: 331 us, six products of 512 cycles a tile.)
 // The running maximum moves only when a row's maximum has grown by more than 2^8 (then O is read, scaled and written
 // back by the row's thread); weights then stay below 2^8 and sums keep fp32's full precision.
 //
 // Warp 0 issues the copies (a ring of K and V tiles, 128-byte swizzle), warp 1 owns TMEM and issues the products, warps
 // 2..9 form the weights, 32 rows a warp.  (Two threads per row, a half of each tile's keys each, had to hand the maximum from
-// one to the other: 269 instead of 253 us for 64 nodes, 190 instead of 187 for 32, and the two-block kernel spilled.  One chain for
-// one row block: 163 instead of 159 us with 1 node, 200 instead of 187 with 32.)
+// one to the other: 190 instead of 187 us for 32 nodes.  One chain: 163 instead of 159 us with 1 node, 200 instead of 187 with
+// 32.)
 //
-// What bounds it, over two full contexts of 119156 rows and 8 cache heads (979 MB, 149.5 us at 6.55 TB/s), 4 query heads a
-// cache head: one row block takes 159 us with 1 node, 163 with 8, 171 with 16 and 187 with 32: HBM, and with more rows the
-// products and exponentials beside it.  64 nodes, two row blocks: 253 us, and the weights bound it: per tile and warp two times
-// 64 keys of about 1400 cycles, 900 of them the exponentials, which two warps of a scheduler share (2048 cycles a tile),
-// against 2800 cycles of loads.  Exponentials by polynomial for a quarter or half of the keys made it slower, as did forming
-// them ahead of the maximum.
+// What bounds it, over two full contexts of 119157 rows and 8 cache heads (979 MB, 149.5 us at 6.55 TB/s), 4 query heads a
+// cache head: 164 us with 1 node, 169 with 8, 176 with 16 and 192 with 32: HBM, and with more rows the products and exponentials
+// beside it.  64 nodes, two row blocks: 318 us, 3000 cycles a tile and block.  The products need 1536 of them and the exponentials
+// 1024; the rest is the hand-over between a chain's products and its weights.
+//
+// At 168 registers a thread (320 threads) the kernel spills 172 bytes and loads 260 again for head_dim 128, about 14 loads
+// from local memory a tile and warp.
 //
 // V rows behind a length may hold anything, and 0 * NaN is NaN: the softmax warps clear them in shared memory before the
 // product.  In a drafted tile, values of V out of range are replaced by zeros and their nodes noted; a row that sees such
@@ -48,10 +48,10 @@ constexpr int kTileKeys = 128, kBlockRows = 128;
 constexpr float kGrow = 8.0f;     // octaves a maximum may grow before O is rescaled
 constexpr int kOCol = 256;        // TMEM columns: S 0..255, O 256 + 128 * chain
 
-template <int D, int MT> struct Shape {
+template <int D> struct Shape {
   static constexpr int kTileBytes = kTileKeys * D * 2;
   static constexpr int kHalfBytes = kTileKeys * 128;                 // 64 columns of a tile
-  static constexpr int kQBytes = MT * kBlockRows * D * 2;
+  static constexpr int kQBytes = kBlockRows * D * 2;
   static constexpr int kStages = (208 * 1024 - kQBytes) / kTileBytes > 8 ? 8 : (208 * 1024 - kQBytes) / kTileBytes;
   static constexpr int kThreads = 64 + 256;
   static constexpr size_t kSmem = kQBytes + (size_t)kStages * kTileBytes + 1024;
@@ -59,9 +59,8 @@ template <int D, int MT> struct Shape {
 
 struct Barriers {
   uint64_t full[8], empty[8], q_full;
-  // [chain], and the half of the keys (scores of one row block: both in [0])
-  uint64_t s_full[2][2], p_ready[2][2], o_done[2][2];
-  uint64_t joined[4];                       // one row block: both chains' maximum and sum of 32 rows are in `ml`
+  uint64_t s_full[2], p_ready[2][2], o_done[2][2];   // [chain][half of the keys]
+  uint64_t joined[4];                       // both chains' maximum and sum of 32 rows are in `ml`
   // ... [segment's parity][chain][row].  One buffer a parity: a warp whose chain has no tile of the next segment waits for
   // nothing before it writes that segment's, while its partner may still be about to read this one's; two segments on,
   // the `joined` between them has passed, which the partner signals behind its read.
@@ -250,10 +249,10 @@ __device__ __forceinline__ void st32(void *dst, const uint32_t *v) {
 struct Maps { CUtensorMap ck, cv, tk, tv; };
 struct Coord { int32_t ck_head, ck_seq, cv_head, cv_seq, tk_head, tk_seq, tv_head, tv_seq; };   // 0 where a dimension is broadcast
 
-template <int D, int MT>
-__global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
+template <int D>
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1)
 tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p, const __grid_constant__ Coord co) {
-  using S = Shape<D, MT>;
+  using S = Shape<D>;
   constexpr int HALVES = D / 64;
   pdl_launch_dependents();
   extern __shared__ unsigned char smem_raw[];
@@ -266,8 +265,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) { mbar_init(&bar.full[i], 1); mbar_init(&bar.empty[i], 1); }
-    for (int i = 0; i < 4; ++i) { mbar_init(&bar.s_full[i >> 1][i & 1], 1); mbar_init(&bar.p_ready[i >> 1][i & 1], 4); mbar_init(&bar.o_done[i >> 1][i & 1], 1); }
-    for (int i = 0; i < 4; ++i) mbar_init(&bar.joined[i], 2);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.s_full[i], 1);
+    for (int i = 0; i < 4; ++i) { mbar_init(&bar.p_ready[i >> 1][i & 1], 4); mbar_init(&bar.o_done[i >> 1][i & 1], 1); mbar_init(&bar.joined[i], 2); }
     mbar_init(&bar.q_full, 8);
     bar.give_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -322,8 +321,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     }
   } else if (warp == 1) {
     // ---- products: the whole warp walks along, so that descriptors stay in uniform registers; one lane issues ----------------
-    constexpr int kScoreKeys = MT == 1 ? kTileKeys : kTileKeys / 2;            // keys of one scores product
-    constexpr uint32_t kIdescS = umma_idesc_bf16_k(128, kScoreKeys);
+    constexpr uint32_t kIdescS = umma_idesc_bf16_k(128, kTileKeys);
     constexpr uint32_t kIdescO = umma_idesc_bf16_k(128, D) | (1u << 16);       // B (the values) MN-major
     const uint32_t leader = elect_one();
     const uint64_t q_desc = umma_desc_k_sw128(saddr(qs), 1024), k_desc = umma_desc_k_sw128(saddr(stages), 1024);
@@ -333,15 +331,15 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       quit();
       return false;
     };
-    // (Addresses in descriptors count 16 bytes.)  `i`: ring index of the tile; x: its scores' buffer; part: which kScoreKeys.
-    const auto scores = [&](int i, int m, int x, int part) {
-      const uint64_t kd = k_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes + part * kScoreKeys * 128) >> 4), qd = q_desc + (uint64_t)(m * ((kBlockRows * D * 2) >> 4));
+    // (Addresses in descriptors count 16 bytes.)  `i`: ring index of the tile; x: its scores' buffer.
+    const auto scores = [&](int i, int x) {
+      const uint64_t kd = k_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes) >> 4);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const uint64_t off = ((ks >> 2) * S::kHalfBytes + (ks & 3) * 32) >> 4;
-        umma_ss(tmem + x * 128 + part * kScoreKeys, qd + off, kd + off, kIdescS, ks > 0, leader);
+        umma_ss(tmem + x * 128, q_desc + off, kd + off, kIdescS, ks > 0, leader);
       }
-      commit(&bar.s_full[x][part], leader);
+      commit(&bar.s_full[x], leader);
     };
     // the product of one half of a tile's keys with the values, as soon as its weights are there
     const auto values = [&](int i, int x, int half, uint32_t parity, bool fresh) {
@@ -350,14 +348,9 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       const uint64_t vd = v_desc + (uint64_t)(((i % S::kStages) * S::kTileBytes + half * 64 * 128) >> 4);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
-        const bool add = !(fresh && half == 0 && ks == 0);
-        if constexpr (MT == 1) {         // per 32 keys: 16 columns of high parts, 16 of low parts
-          const uint32_t at = a + (ks >> 1) * 32 + (ks & 1) * 8;
-          umma_ts(d, at, vd + ks * (2048 >> 4), kIdescO, add, leader);
-          umma_ts(d, at + 16, vd + ks * (2048 >> 4), kIdescO, 1, leader);
-        } else {
-          umma_ts(d, a + ks * 8, vd + ks * (2048 >> 4), kIdescO, add, leader);
-        }
+        const uint32_t at = a + (ks >> 1) * 32 + (ks & 1) * 8;   // per 32 keys: 16 columns of high parts, 16 of low parts
+        umma_ts(d, at, vd + ks * (2048 >> 4), kIdescO, !(fresh && half == 0 && ks == 0), leader);
+        umma_ts(d, at + 16, vd + ks * (2048 >> 4), kIdescO, 1, leader);
       }
       commit(&bar.o_done[x][half], leader);
       return true;
@@ -369,43 +362,26 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       const int n = w.t1 - w.t0;
       bool ok = ready(&bar.q_full, seg & 1) && arrived(i);
       if (!ok) break;
-#pragma unroll
-      for (int k = 0; k < (MT == 1 ? 1 : 4); ++k) scores(i, k >> 1, MT == 1 ? cnt & 1 : k >> 1, k & 1);
+      scores(i, cnt & 1);
       release(i);
       for (int t = 0; t < n; ++t, ++cnt, i += 2) {
-        const bool more = t + 1 < n;
-        if constexpr (MT == 1) {
-          if (more) {
-            if (!(ok = arrived(i + 2))) break;
-            scores(i + 2, 0, (cnt + 1) & 1, 0);
-            release(i + 2);
-          }
-          const uint32_t parity = (cnt >> 1) & 1;
-          if (!(ok = arrived(i + 1) && values(i + 1, cnt & 1, 0, parity, t < 2) && values(i + 1, cnt & 1, 1, parity, t < 2))) break;
-        } else {
-          if (!(ok = arrived(i + 1))) break;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {    // (row block, half): the scores of the next tile replace weights that are used
-            if (!(ok = ok && values(i + 1, k >> 1, k & 1, cnt & 1, t == 0))) continue;
-            if (more) {
-              if (k == 0 && !(ok = arrived(i + 2))) continue;
-              scores(i + 2, k >> 1, k >> 1, k & 1);
-            }
-          }
-          if (!ok) break;
-          if (more) release(i + 2);
+        if (t + 1 < n) {
+          if (!(ok = arrived(i + 2))) break;
+          scores(i + 2, (cnt + 1) & 1);
+          release(i + 2);
         }
+        const uint32_t parity = (cnt >> 1) & 1;
+        if (!(ok = arrived(i + 1) && values(i + 1, cnt & 1, 0, parity, t < 2) && values(i + 1, cnt & 1, 1, parity, t < 2))) break;
         release(i + 1);
       }
       if (!ok) break;
     }
   } else {
     // ---- weights: a thread per query row -------------------------------------------------------------------------------------
-    const int chain = (warp - 2) >> 2, m = MT == 1 ? 0 : chain;                              // row block
-    const int quarter = warp & 3, r_in = quarter * 32 + lane, row = m * kBlockRows + r_in;   // TMEM lanes 32 * (warp % 4)..
+    const int chain = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;        // TMEM lanes 32 * (warp % 4)..
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16), o_base = lane_base + kOCol + chain * 128;
     const int g = group_row(p, row0 + row), node = row0 + row - g * p.nodes;                // query head in the group, node
-    const bool real = row < n_rows, warp_real = m * kBlockRows + quarter * 32 < n_rows;
+    const bool real = row < n_rows, warp_real = quarter * 32 < n_rows;
     int cnt = 0, i0 = 0, seg = 0;                        // tiles done, ring index of the segment's first K, segments done
     const auto signal = [&](uint64_t *b) {               // one arrival for the warp, behind all of its lanes' writes
       __syncwarp();
@@ -413,14 +389,14 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
     };
     for (; w.valid() && !*give_up; w.next(p), ++seg) {
       // the block's queries, for the K-major swizzled operand (rows that do not exist: zeros); all loads in flight at once
-      constexpr int kLoaders = MT == 1 ? 256 : 128, kLoads = kBlockRows * (D / 8) / kLoaders;
+      constexpr int kLoaders = 256, kLoads = kBlockRows * (D / 8) / kLoaders;
+      const int first = chain * 128 + quarter * 32 + lane;
       uint4 qv[kLoads];
       {
         const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(p.q) + w.b * p.q_stride[0] + (int64_t)(w.head * per_head) * p.q_stride[1];
-        const int first = (MT == 1 ? chain * 128 : 0) + quarter * 32 + lane;
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
-          const int e = first + k * kLoaders, r = m * kBlockRows + e / (D / 8), c = e % (D / 8);
+          const int e = first + k * kLoaders, r = e / (D / 8), c = e % (D / 8);
           const int gr = group_row(p, row0 + r);
           qv[k] = make_uint4(0, 0, 0, 0);
           if (r < n_rows) qv[k] = ld16(q + gr * p.q_stride[1] + (int64_t)(row0 + r - gr * p.nodes) * p.q_stride[2] + c * 8);
@@ -453,12 +429,10 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       };
       if (warp_real && w.t1 > w.ctiles) look(max(w.t0 - w.ctiles, 0) * kTileKeys);   // ahead of its use
       {
-        unsigned char *dst = qs + m * (kBlockRows * D * 2);
-        const int first = (MT == 1 ? chain * 128 : 0) + quarter * 32 + lane;
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
           const int e = first + k * kLoaders, r = e / (D / 8), c = e % (D / 8);
-          *reinterpret_cast<uint4 *>(dst + (c >> 3) * (kBlockRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = qv[k];
+          *reinterpret_cast<uint4 *>(qs + (c >> 3) * (kBlockRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = qv[k];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         signal(&bar.q_full);
@@ -466,9 +440,9 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
       float top = -INFINITY, sum = 0.0f;                 // maximum in use, in octaves; sum of this thread's weights
       const int n_tiles = w.t1 - w.t0, plain = w.len / kTileKeys - w.t0;   // the first `plain` tiles are seen whole
       for (int st = 0; st < n_tiles; ++st, ++cnt) {
-        if (MT == 1 && (cnt & 1) != chain) continue;     // the other chain's tile
-        const int x = chain;
-        const uint32_t parity = MT == 1 ? (cnt >> 1) & 1 : cnt & 1;
+        if ((cnt & 1) != chain) continue;                // the other chain's tile
+        const uint32_t parity = (cnt >> 1) & 1;
+        if (!await(&bar.s_full[chain], parity)) { quit(); break; }
         const bool masked = st >= plain;
         int n_keys = kTileKeys, dt = -1;                 // filled keys of the tile; drafted tile
         if (masked) {
@@ -478,17 +452,16 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         }
         const bool drafted = dt >= 0;
         // values that must not meet the product: rows of the cache behind the length, drafted rows out of range
-        if (masked && m == 0) {
+        if (masked) {
           // (the scores are there once every warp has left the segment before, whose marks in `odd` these replace)
-          if (!await(&bar.s_full[x][0], parity)) { quit(); break; }
           const int i = i0 + 2 * st;
           const int vi = (i + 1) % S::kStages;
           unsigned char *vt = stages + (size_t)vi * S::kTileBytes;
           if (!await(&bar.full[vi], ((i + 1) / S::kStages) & 1)) { quit(); break; }
           // this thread's row of the tile, 16 bytes at a time (in an order that keeps the banks apart)
-          const auto piece = [&](int c) { return reinterpret_cast<uint4 *>(vt + (c >> 3) * S::kHalfBytes + r_in * 128 + (((c + lane) & 7) << 4)); };
+          const auto piece = [&](int c) { return reinterpret_cast<uint4 *>(vt + (c >> 3) * S::kHalfBytes + row * 128 + (((c + lane) & 7) << 4)); };
           bool odd = false;
-          if (r_in >= n_keys) {
+          if (row >= n_keys) {                           // (as a key of the tile)
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) *piece(c) = make_uint4(0, 0, 0, 0);
           } else if (drafted) {
@@ -523,9 +496,8 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
         bool ok = true;
 #pragma unroll
         for (int half = 0; half < 2 && ok; ++half) {
-          if ((MT == 2 || half == 0) && !(ok = await(&bar.s_full[x][half], parity))) break;
           fence_after();
-          const uint32_t s_base = lane_base + x * 128 + half * 64;
+          const uint32_t s_base = lane_base + chain * 128 + half * 64;
           if (warp_real) {
             uint32_t v[32], u[32];
             load32_async(s_base, v);
@@ -542,9 +514,9 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             const bool move = now > top + kGrow || (top == -INFINITY && now > -INFINITY);
             if (__any_sync(0xFFFFFFFFu, move)) {
               const float use = move ? now : top, fade = move ? exp2_fast(top - use) : 1.0f;
-              if (half == 1 || st >= (MT == 1 ? 2 : 1)) {
+              if (half == 1 || st >= 2) {
                 // O holds the chain's products up to the half before: that one has to be in it
-                if (!(ok = await(&bar.o_done[x][half ^ 1], half == 1 ? parity : parity ^ 1))) break;
+                if (!(ok = await(&bar.o_done[chain][half ^ 1], half == 1 ? parity : parity ^ 1))) break;
                 fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D; c += 8) scale8(o_base + c, fade);
@@ -556,56 +528,41 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             uint64_t sum2 = 0;
             weigh(v, c2, minus2, sum2);
             weigh(u, c2, minus2, sum2);
-            if constexpr (MT == 1) {
-              store_two_parts(v, s_base);
-              store_two_parts(u, s_base + 32);
-            } else {
-              uint32_t o[32];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                o[j] = pack_bf16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
-                o[16 + j] = pack_bf16(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
-              }
-              store32(s_base, o);
-            }
+            store_two_parts(v, s_base);
+            store_two_parts(u, s_base + 32);
             sum += low_of(sum2) + high_of(sum2);
           }
           store_wait();
           fence_before();
-          signal(&bar.p_ready[x][half]);
+          signal(&bar.p_ready[chain][half]);
         }
         if (!ok) { quit(); break; }
       }
       i0 += 2 * n_tiles;
       if (*give_up) break;
       // (a segment of one tile leaves the chain that had none without an O)
-      const bool last_mine = MT == 2 || ((cnt - 1) & 1) == chain, mine = last_mine || n_tiles > 1;
+      const bool last_mine = ((cnt - 1) & 1) == chain, mine = last_mine || n_tiles > 1;
       if (mine) {
         const int last = last_mine ? cnt - 1 : cnt - 2;
-        if (!await(&bar.o_done[chain][1], (MT == 1 ? last >> 1 : last) & 1)) { quit(); break; }
+        if (!await(&bar.o_done[chain][1], (last >> 1) & 1)) { quit(); break; }
         fence_after();
       }
-      if constexpr (MT == 1) {                           // each chain's O and statistics for the other's warp of the same rows
-        bar.ml[seg & 1][chain][r_in] = make_float2(top, sum);
-        fence_before();
-        signal(&bar.joined[quarter]);
-        if (!await(&bar.joined[quarter], seg & 1)) { quit(); break; }
-        fence_after();
-      }
+      // each chain's O and statistics for the other's warp of the same rows
+      bar.ml[seg & 1][chain][row] = make_float2(top, sum);
+      fence_before();
+      signal(&bar.joined[quarter]);
+      if (!await(&bar.joined[quarter], seg & 1)) { quit(); break; }
+      fence_after();
       // ---- the segment's rows: finished, or a partial -------------------------------------------------------------------------
       if (warp_real) {
-        float fade = 1.0f, other_fade = 0.0f;            // one row block: factors on the two chains' O
-        if constexpr (MT == 1) {
-          const float2 other = bar.ml[seg & 1][chain ^ 1][r_in];
-          const float both = fmaxf(top, other.x);
-          fade = top == both ? 1.0f : exp2_fast(top - both);
-          other_fade = other.x == both ? 1.0f : exp2_fast(other.x - both);
-          sum = sum * fade + other.y * other_fade;
-          top = both;
-        }
-        const bool others = MT == 1 && (n_tiles > 1 || !mine);
-        constexpr int kCols = MT == 1 ? D / 2 : D;       // columns of a thread: a row's two chains share them
-        const int c0 = MT == 1 ? chain * kCols : 0;
+        const float2 other = bar.ml[seg & 1][chain ^ 1][row];
+        const float both = fmaxf(top, other.x);
+        const float fade = top == both ? 1.0f : exp2_fast(top - both), other_fade = other.x == both ? 1.0f : exp2_fast(other.x - both);
+        sum = sum * fade + other.y * other_fade;
+        top = both;
+        const bool others = n_tiles > 1 || !mine;
+        constexpr int kCols = D / 2;                     // columns of a thread: a row's two chains share them
+        const int c0 = chain * kCols;
         const bool whole = w.whole();
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int64_t at = ((int64_t)w.b * p.q_heads + w.head * per_head + g) * p.nodes + node;
@@ -618,13 +575,11 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
           const int c = c0 + cc;
           uint32_t v[32];
           if (mine) load32(o_base + c, v);
-          if constexpr (MT == 1) {
-            uint32_t u[32];
-            if (others) load32(lane_base + kOCol + (chain ^ 1) * 128 + c, u);
+          uint32_t u[32];
+          if (others) load32(lane_base + kOCol + (chain ^ 1) * 128 + c, u);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              v[e] = __float_as_uint((mine ? __uint_as_float(v[e]) * fade : 0.0f) + (others ? __uint_as_float(u[e]) * other_fade : 0.0f));
-          }
+          for (int e = 0; e < 32; ++e)
+            v[e] = __float_as_uint((mine ? __uint_as_float(v[e]) * fade : 0.0f) + (others ? __uint_as_float(u[e]) * other_fade : 0.0f));
           if (any_odd && real) {
             // values out of range of the nodes this row sees, in the tiles of this segment
             for (int dt = max(w.t0 - w.ctiles, 0); dt < w.t1 - w.ctiles; ++dt)
@@ -655,7 +610,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
             }
           }
         }
-        if (real && (MT == 2 || chain == 0)) {
+        if (real && chain == 0) {
           if (!whole) p.part_ml[slot] = make_float2(top, sum);
           else if (p.lse) p.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
         }
@@ -687,8 +642,8 @@ int make_map(CUtensorMap *map, const void *base, int D, int64_t rows, int64_t he
   return LRQK_OK;
 }
 
-template <int D, int MT> int launch(const Params &p, cudaStream_t stream) {
-  using S = Shape<D, MT>;
+template <int D> int launch(const Params &p, cudaStream_t stream) {
+  using S = Shape<D>;
   Maps maps;
   Coord co;
   int rc = make_map(&maps.tk, p.tree_k, D, p.nodes, p.tree_heads, p.batch, p.tk_stride, co.tk_head, co.tk_seq);
@@ -702,7 +657,7 @@ template <int D, int MT> int launch(const Params &p, cudaStream_t stream) {
     co.ck_head = co.cv_head = co.ck_seq = co.cv_seq = 0;
   }
   if (rc != LRQK_OK) return rc;
-  auto kern = tree_tc_kernel<D, MT>;
+  auto kern = tree_tc_kernel<D>;
   static SmemOptIn opt_in;
   LRQK_CUDA_TRY(opt_in.ensure(kern, S::kSmem));
   LRQK_CUDA_TRY(launch_dependent(kern, dim3((unsigned)(p.groups * p.row_blocks)), dim3(S::kThreads), S::kSmem, stream, 0, maps, p, co));
@@ -711,19 +666,17 @@ template <int D, int MT> int launch(const Params &p, cudaStream_t stream) {
 
 }  // namespace
 
-// One block of 128 rows where the rows of a cache head fit it, two of them above; one CTA an SM.
-bool plan_tc(Params &p) {
-  p.rows_per_block = p.rows <= kBlockRows ? kBlockRows : 2 * kBlockRows;
+// Blocks of 128 rows; one CTA an SM, more than that only where there are more blocks than SMs.
+void plan_tc(Params &p) {
+  p.rows_per_block = kBlockRows;
   p.tile_keys = kTileKeys;
   p.unit_cost = 4;
   p.row_blocks = (p.rows + p.rows_per_block - 1) / p.rows_per_block;
-  p.groups = kNumSMs / p.row_blocks;
-  return p.groups >= 1;
+  p.groups = p.row_blocks < kNumSMs ? kNumSMs / p.row_blocks : 1;
 }
 
 int launch_tc(const Params &p, cudaStream_t stream) {
-  if (p.rows_per_block == kBlockRows) return p.head_dim == 64 ? launch<64, 1>(p, stream) : launch<128, 1>(p, stream);
-  return p.head_dim == 64 ? launch<64, 2>(p, stream) : launch<128, 2>(p, stream);
+  return p.head_dim == 64 ? launch<64>(p, stream) : launch<128>(p, stream);
 }
 
 }  // namespace tree

@@ -147,7 +147,7 @@ __device__ __forceinline__ bool sees(const Params &p, int b, int node, int j) {
 }
 
 int launch_tc(const Params &p, cudaStream_t stream);     // bf16: tcgen05 kernel (tree_attention_tc.cu)
-bool plan_tc(Params &p);
+void plan_tc(Params &p);
 
 }  // namespace tree
 }  // namespace lrqk
