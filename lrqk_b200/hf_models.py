@@ -32,7 +32,8 @@ for those heads only and all-gathered, and ``cache.attend`` returns all heads' r
 exchange fused into the attention kernel.
 
 With ``cache.drafting(mask)`` open, a decoding layer takes several tokens a call -- a drafted tree -- and attends them
-with ``cache.attend_tree``; the states change when ``cache.accept`` decodes the tokens that were right.
+with ``cache.attend_tree``; the states change when ``cache.accept`` decodes the tokens that were right.  A layer that is not
+decoding yet refuses.
 
 ``patch_model(model, fused_rotary=True)`` rotates q and k of prompts and drafts with ``rotary.apply_rotary`` (one launch,
 angles right at far positions, one rounding) instead of the family's eager function; off, results are those of that function.
@@ -127,6 +128,9 @@ def lrqk_attention_forward(self, hidden_states: torch.Tensor,
         return self._lrqk_original_forward(hidden_states, position_embeddings=position_embeddings,
                                            attention_mask=attention_mask, past_key_values=past_key_values, **kwargs)
     cache: DynamicLRQKCache = past_key_values
+    if cache.is_drafting and not cache.is_decoding(self.layer_idx):
+        raise RuntimeError("drafting() needs layers that are decoding; this one's prompt is shorter than num_active_tokens so far: "
+                           "take its tokens one by one until it is full")
     input_shape = hidden_states.shape[:-1]
     hidden_shape = (*input_shape, -1, self.head_dim)
     if hidden_states.shape[1] == 1 and cache.is_decoding(self.layer_idx) and not cache.is_drafting:
@@ -155,7 +159,7 @@ def lrqk_attention_forward(self, hidden_states: torch.Tensor,
         query_states, key_states = rope(query_states, key_states, cos, sin)
 
     q_len = query_states.shape[2]
-    if cache.is_decoding(self.layer_idx) and cache.is_drafting:
+    if cache.is_drafting:
         attn_output = cache.attend_tree(query_states, key_states, value_states, self.layer_idx).transpose(1, 2)
     elif cache.is_decoding(self.layer_idx):
         if q_len != 1:

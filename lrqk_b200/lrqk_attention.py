@@ -916,7 +916,7 @@ class DynamicLRQKCache(_CacheBase):
                layer_idx: int, attention_mask: Optional[torch.Tensor] = None):
         if any(c is None for c in (query_states, key_states, value_states)):
             raise ValueError("None of query_states, key_states, and value_states can be None")
-        self._drafted = {}
+        self._follow_on("update")
         if self.sharding is not None:
             query_states, key_states, value_states, attention_mask = self._local(query_states, key_states,
                                                                                  value_states, attention_mask)
@@ -927,7 +927,7 @@ class DynamicLRQKCache(_CacheBase):
     def attend(self, query_states: torch.Tensor, key_states: torch.Tensor, value_states: torch.Tensor,
                layer_idx: int) -> torch.Tensor:
         """Decode-state only: one step plus attention, returns [B,Hq,1,d]."""
-        self._drafted = {}                                       # a draft made before this token no longer follows the context
+        self._follow_on("attend")
         if self.sequence_state[layer_idx] != self.State.decoding:
             raise RuntimeError("attend() is only valid once the layer is decoding; use update() before")
         fac = self.lwattn[layer_idx]
@@ -944,7 +944,7 @@ class DynamicLRQKCache(_CacheBase):
         """``attend`` from the fused projection of the new token: qkv [B, 1, (q_heads + 2 kv_heads) d] holds the
         un-rotated q, k and v heads of the whole model, cos / sin [B or 1, 1, d] the position's rotary factors.
         One kernel rotates q and k and cuts out this rank's heads; returns the rows of all heads [B,Hq,1,d]."""
-        self._drafted = {}
+        self._follow_on("attend_qkv")
         if self.sequence_state[layer_idx] != self.State.decoding:
             raise RuntimeError("attend_qkv() is only valid once the layer is decoding; use update() before")
         fac, bsz = self.lwattn[layer_idx], qkv.shape[0]
@@ -957,6 +957,12 @@ class DynamicLRQKCache(_CacheBase):
         fac.decode_attend_push(q, k, v, exchange)
         return self.sharding.gather_step(bsz, kv_heads, q_heads).unsqueeze(2)
 
+    def _follow_on(self, what: str):
+        """Before a call that adds tokens to the context."""
+        if self._draft is not None:
+            raise RuntimeError(f"{what}() inside drafting(): a draft adds no tokens to the context")
+        self._drafted = {}                                       # a draft made before no longer follows the context
+
     # ---- drafted tokens ---------------------------------------------------------------------------
     # (The reference decodes one token a call, :1506-1613; this is what verifying a draft needs on top.)
     @contextlib.contextmanager
@@ -964,7 +970,8 @@ class DynamicLRQKCache(_CacheBase):
         """While this is open, a decoding layer takes several tokens a call as a drafted tree: the patched model's
         forward (``input_ids`` [B,T], ``position_ids`` of the nodes' depths) attends them with ``attend_tree`` under
         ``mask`` (``tree_mask(parents)``; ``None``: a chain) and changes no layer's state.  ``accept`` then takes the
-        tokens that were right."""
+        tokens that were right.  Calls that would add tokens are refused meanwhile; so is a forward while the layers are
+        not decoding yet (a prompt shorter than ``num_active_tokens`` goes on token by token until they are)."""
         if self.sharding is not None:
             raise NotImplementedError("drafted tokens on a head-sharded cache")
         if self._draft is not None:
