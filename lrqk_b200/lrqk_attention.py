@@ -848,6 +848,7 @@ class DynamicLRQKCache(_CacheBase):
         self.sharding = None
         self._draft = None                                       # (mask,) while drafting() is open
         self._drafted: Dict[int, tuple] = {}                     # q, k, v of the last draft, per layer
+        self._draft_mask = None                                  # (mask,) of the last draft
 
     def shard_heads(self, group=None, sharding=None):
         """Run every layer for this rank's share of the (batch x KV head) units only (one process per
@@ -976,7 +977,9 @@ class DynamicLRQKCache(_CacheBase):
             raise NotImplementedError("drafted tokens on a head-sharded cache")
         if self._draft is not None:
             raise RuntimeError("a draft is open already")
-        self._draft, self._drafted = (mask,), {}
+        if mask is not None:
+            mask = mask.clone()                                  # (accept looks at it, the caller may reuse its own)
+        self._draft, self._drafted, self._draft_mask = (mask,), {}, (mask,)
         try:
             yield self
         except BaseException:
@@ -1003,7 +1006,8 @@ class DynamicLRQKCache(_CacheBase):
     def accept(self, nodes) -> None:
         """Decode the last draft's ``nodes`` (indices along one path from the root, the same for every sequence) into
         every layer, in order, from the q, k, v of the drafting call: ring write, projection, selection and fetch as
-        for any decoded token, without a forward of the model.  The draft is used up."""
+        for any decoded token, without a forward of the model.  Each of them has to see the accepted ones up to itself and
+        no other node (a chain without a mask); a look at the mask waits for the device.  The draft is used up."""
         if self._draft is not None:
             raise RuntimeError("accept() after drafting() is closed")
         if not self._drafted:
@@ -1012,10 +1016,26 @@ class DynamicLRQKCache(_CacheBase):
         t = next(iter(self._drafted.values()))[0].shape[2]
         if any(not 0 <= i < t for i in nodes) or any(b <= a for a, b in zip(nodes, nodes[1:])):
             raise ValueError(f"nodes {nodes}: ascending indices below {t} are expected")
+        if nodes and self._draft_mask is not None:
+            self._check_path(nodes, t, self._draft_mask[0])
         drafted, self._drafted = self._drafted, {}               # an error half-way leaves nothing to decode twice
         for layer_idx, (q, k, v) in drafted.items():
             for i in nodes:
                 self.lwattn[layer_idx]._decode(q[:, :, i:i + 1], k[:, :, i:i + 1], v[:, :, i:i + 1], attention=False)
+
+    @staticmethod
+    def _check_path(nodes, t: int, mask: Optional[torch.Tensor]):
+        """Accepted nodes form one path from a root, for every sequence: node i of the path sees the path up to itself."""
+        if mask is None:
+            if nodes != list(range(len(nodes))):
+                raise ValueError(f"nodes {nodes}: not a path of the draft, which was a chain (no mask)")
+            return
+        want = torch.zeros(len(nodes), t, dtype=torch.bool)
+        for i, node in enumerate(nodes):
+            want[i:, node] = True
+        for b, seen in enumerate(mask.cpu().reshape(-1, t, t)):
+            if not torch.equal(seen[nodes] != 0, want):
+                raise ValueError(f"nodes {nodes}: not a path of the draft's tree from a root" + (f" (sequence {b})" if mask.dim() == 3 else ""))
 
     def state_dict(self) -> dict:
         """The whole cache for ``load_state_dict``: every decoding layer's ``state_dict()`` and the prompt rows of

@@ -67,3 +67,80 @@ def test_nothing_commits_a_token_while_a_draft_is_open():
     assert bool((k == 1).all()) and not cache.temp_buff_cache_qkv
     cache.update(q, k, k, 0)
     assert len(cache.temp_buff_cache_qkv[0]) == 5
+
+
+class _Layer:
+    """A decoding layer that counts."""
+
+    def __init__(self, fails=False):
+        self.taken = []
+
+    def attend_tree(self, q, k, v, mask):
+        return torch.zeros_like(q)
+
+    def _decode(self, q, k, v, attention):
+        self.taken.append(float(q.flatten()[0]))
+
+    def close(self):
+        pass
+
+
+def _drafted(mask, nodes, layers=2, batch=1):
+    cache = _cache()
+    cache.lwattn = {i: _Layer() for i in range(layers)}
+    q = torch.arange(float(nodes))[None, None, :, None].expand(batch, 1, nodes, 16)
+    for i in range(layers):
+        cache.sequence_state[i] = DynamicLRQKCache.State.decoding
+    with cache.drafting(mask):
+        for i in range(layers):
+            cache.attend_tree(q, q, q, i)
+    return cache
+
+
+PARENTS = [-1, 0, 0, 1, 1, 2, -1, 6]
+PATHS = [[], [0], [0, 1], [0, 2], [0, 1, 4], [0, 2, 5], [6], [6, 7]]
+NO_PATHS = [[1], [1, 2], [4], [0, 4], [0, 1, 2], [0, 1, 3, 4], [0, 6], [6, 0], [7], [0, 0], [5]]
+
+
+@pytest.mark.parametrize("form", ["bool", "uint8", "per sequence"])
+def test_accept_takes_paths_of_the_tree_only(form):
+    mask = tree_mask(PARENTS)
+    if form == "uint8":
+        mask = mask.to(torch.uint8) * 5
+    if form == "per sequence":
+        mask = torch.stack([mask, mask])
+    cache = _drafted(mask, len(PARENTS))
+    for bad in NO_PATHS + [[0, 8], [-1]]:
+        with pytest.raises(ValueError):
+            cache.accept(bad)
+    assert not cache.lwattn[0].taken and cache._drafted                 # refused before any layer changed, and still there
+    for path in PATHS:
+        cache = _drafted(mask, len(PARENTS))
+        cache.accept(path)
+        assert cache.lwattn[0].taken == cache.lwattn[1].taken == [float(i) for i in path]
+
+
+def test_accept_of_a_chain_and_of_trees_that_differ():
+    for nodes, good in (([0], True), ([0, 1, 2], True), ([1], False), ([0, 2], False)):
+        cache = _drafted(None, 4)
+        if good:
+            cache.accept(nodes)
+        else:
+            with pytest.raises(ValueError):
+                cache.accept(nodes)
+    masks = tree_mask([[-1, 0, 0], [-1, 0, 1]])
+    cache = _drafted(masks, 3, batch=2)
+    with pytest.raises(ValueError, match="sequence 1"):
+        cache.accept([0, 2])                                            # a path of the first sequence's tree alone
+    cache.accept([0, 1])
+    assert cache.lwattn[0].taken == [0.0, 1.0]
+
+
+def test_a_mask_that_the_caller_reuses_is_the_drafts_own():
+    mask = tree_mask([-1, 0, 0])
+    cache = _drafted(mask, 3)
+    mask.copy_(tree_mask([-1, 0, 1]))
+    with pytest.raises(ValueError):
+        cache.accept([0, 1, 2])
+    cache.accept([0, 2])
+    assert cache.lwattn[0].taken == [0.0, 2.0]
