@@ -1012,6 +1012,9 @@ class DynamicLRQKCache(_CacheBase):
             raise RuntimeError("accept() after drafting() is closed")
         if not self._drafted:
             raise RuntimeError("no drafted tokens to accept")
+        missing = [i for i, state in self.sequence_state.items() if state == self.State.decoding and i not in self._drafted]
+        if missing:
+            raise RuntimeError(f"layers {missing} took no part in the draft: nothing can be accepted")
         nodes = [int(i) for i in nodes]
         t = next(iter(self._drafted.values()))[0].shape[2]
         if any(not 0 <= i < t for i in nodes) or any(b <= a for a, b in zip(nodes, nodes[1:])):

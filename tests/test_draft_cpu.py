@@ -144,3 +144,17 @@ def test_a_mask_that_the_caller_reuses_is_the_drafts_own():
         cache.accept([0, 1, 2])
     cache.accept([0, 2])
     assert cache.lwattn[0].taken == [0.0, 2.0]
+
+
+def test_a_draft_that_reached_some_layers_only_cannot_be_accepted():
+    cache = _drafted(None, 3)
+    q = torch.zeros(1, 1, 3, 16)
+    with cache.drafting():
+        cache.attend_tree(q, q, q, 0)
+        try:
+            raise KeyError("an error between two layers, caught inside")
+        except KeyError:
+            pass
+    with pytest.raises(RuntimeError, match=r"\[1\]"):
+        cache.accept([0])
+    assert not cache.lwattn[0].taken
