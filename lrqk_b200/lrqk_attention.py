@@ -1062,6 +1062,7 @@ class DynamicLRQKCache(_CacheBase):
                     num_key_value_groups=self.num_key_value_groups)
         if sd["settings"] != mine:
             raise ValueError(f"the saved cache was configured as {sd['settings']}, this one as {mine}")
+        self._follow_on("load_state_dict")
         for idx, entry in sd["layers"].items():
             idx = int(idx)
             if entry["state"] == "decoding":

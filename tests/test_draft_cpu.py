@@ -158,3 +158,20 @@ def test_a_draft_that_reached_some_layers_only_cannot_be_accepted():
     with pytest.raises(RuntimeError, match=r"\[1\]"):
         cache.accept([0])
     assert not cache.lwattn[0].taken
+
+
+def test_a_draft_made_before_a_restore_cannot_be_accepted_onto_it():
+    saved = _cache()
+    x = torch.ones(1, 2, 5, 16)
+    saved.update(torch.ones(1, 4, 5, 16), x, x, 0)
+    sd = saved.state_dict()
+    cache = _drafted(None, 3, layers=1)
+    cache.load_state_dict(sd, device="cpu")
+    with pytest.raises(RuntimeError, match="no drafted"):
+        cache.accept([0])
+    assert not cache.lwattn[0].taken
+    other = _cache()
+    with other.drafting():
+        with pytest.raises(RuntimeError, match="drafting"):
+            other.load_state_dict(sd, device="cpu")
+    assert not other.temp_buff_cache_qkv
