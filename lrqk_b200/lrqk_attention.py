@@ -28,7 +28,7 @@ import torch
 
 from . import _lib
 from .state import HostStore, LayerState, _ptr, _stream, on_device
-from .tree import tree_attention
+from .tree import check_tree_status, tree_attention
 
 try:  # HF is only needed for the Cache base class
     from transformers import cache_utils as _cache_utils
@@ -849,6 +849,7 @@ class DynamicLRQKCache(_CacheBase):
         self._draft = None                                       # (mask,) while drafting() is open
         self._drafted: Dict[int, tuple] = {}                     # q, k, v of the last draft, per layer
         self._draft_mask = None                                  # (mask,) of the last draft
+        self._draft_devices = set()                              # where drafts were attended
 
     def shard_heads(self, group=None, sharding=None):
         """Run every layer for this rank's share of the (batch x KV head) units only (one process per
@@ -1001,6 +1002,7 @@ class DynamicLRQKCache(_CacheBase):
             raise RuntimeError("attend_tree() is only valid once the layer is decoding; use update() before")
         out = self.lwattn[layer_idx].attend_tree(query_states, key_states, value_states, self._draft[0])
         self._drafted[layer_idx] = (query_states, key_states, value_states)
+        self._draft_devices.add(query_states.device)
         return out
 
     def accept(self, nodes) -> None:
@@ -1082,14 +1084,17 @@ class DynamicLRQKCache(_CacheBase):
 
     def check_status(self) -> None:
         """Synchronising check of every layer's device-side status words (the hit/miss difference's mismatch flag,
-        the bounded waits of the attention and projection kernels) and of the exchange's arrival wait; raises
-        LrqkError for the first that is set.  Off the hot path: ``close()`` calls it, a serving loop may call it
+        the bounded waits of the attention and projection kernels), of the exchange's arrival wait and, on the devices
+        where this cache attended drafts, of ``tree_attention`` (one word a device, whoever called; ``check_tree_status``);
+        raises LrqkError for the first that is set.  Off the hot path: ``close()`` calls it, a serving loop may call it
         once per request."""
         for fac in self.lwattn.values():
             if fac.state is not None:
                 fac.state.check_status()
         if self.sharding is not None and self.sharding._exchange is not None:
             self.sharding._exchange.check_status()
+        for device in self._draft_devices:
+            check_tree_status(device)
 
     def close(self, check: bool = True):
         """Free every layer's device and page-locked host memory and the exchange buffers (after a last look at

@@ -175,3 +175,22 @@ def test_a_draft_made_before_a_restore_cannot_be_accepted_onto_it():
         with pytest.raises(RuntimeError, match="drafting"):
             other.load_state_dict(sd, device="cpu")
     assert not other.temp_buff_cache_qkv
+
+
+def test_check_status_and_close_look_at_the_tree_attentions_word(monkeypatch):
+    from lrqk_b200 import _lib, lrqk_attention
+    looked = []
+
+    def look(device):
+        looked.append(device)
+        raise _lib.LrqkError(_lib.ETIMEOUT, "lrqk_tree_attention", "")
+
+    monkeypatch.setattr(lrqk_attention, "check_tree_status", look, raising=False)
+    monkeypatch.setattr(_Layer, "state", None, raising=False)
+    _cache().check_status()                                             # no draft: nothing to look at
+    assert not looked
+    cache = _drafted(None, 3)
+    for call in (cache.check_status, cache.close):
+        with pytest.raises(_lib.LrqkError):
+            call()
+    assert looked == [torch.device("cpu")] * 2

@@ -1,0 +1,34 @@
+"""The status word of the tree attention's bounded waits: who looks at it, and when.  (No wait is made to run out here: the word
+is set by hand.)"""
+import pytest
+import torch
+
+from lrqk_b200 import DynamicLRQKCache, check_tree_status, tree_attention
+from lrqk_b200 import tree as tree_module
+from lrqk_b200._lib import ETIMEOUT, LrqkError
+from test_gpu_tree import check, make
+
+pytestmark = pytest.mark.gpu
+
+
+def _word():
+    q, ck, cv, tk, tv, _ = make(1, 2, 1, 1, 3, 9, 64, torch.bfloat16)
+    tree_attention(q, ck, cv, tk, tv)
+    return tree_module._status[torch.cuda.current_device()]
+
+
+def test_the_cache_reports_it_where_it_reports_the_others():
+    word = _word()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()  # noqa: E731
+    for how in ("check_status", "close"):
+        cache = DynamicLRQKCache(r=16, num_active_tokens=64, lite_tokens=8, max_sequence_length=512, num_key_value_groups=2, init_aq_ak_method="top")
+        cache.update(r(1, 4, 100, 64), r(1, 2, 100, 64), r(1, 2, 100, 64), 0)
+        with cache.drafting():
+            cache.attend_tree(r(1, 4, 3, 64), r(1, 2, 3, 64), r(1, 2, 3, 64), 0)
+        cache.check_status()
+        word[0] = ETIMEOUT
+        with pytest.raises(LrqkError):
+            getattr(cache, how)()
+        cache.check_status()                                       # looked at once
+        cache.close()
