@@ -54,13 +54,18 @@ def _status_word(device: torch.device) -> Optional[int]:
 
 
 def check_tree_status(device=None) -> None:
-    """Synchronising look at the status word of a device's ``tree_attention`` calls: raises ``LrqkError`` if a bounded
-    wait of one ran out (its rows, and those of later calls until this look, are NaN), and clears it."""
+    """Synchronising look at the status word of a device's ``tree_attention`` calls, on whichever stream: raises
+    ``LrqkError`` if a bounded wait of one ran out (its rows, and those of later calls until this look, are NaN), and
+    clears it."""
     index = torch.cuda.current_device() if device is None or torch.device(device).index is None else torch.device(device).index
     word = _status.get(index)
-    if word is not None and int(word[0]) != 0:
-        code = int(word[0])
+    if word is None:
+        return
+    torch.cuda.synchronize(index)                                # calls of other streams than the current one
+    code = int(word[0])
+    if code != 0:
         word.zero_()
+        torch.cuda.synchronize(index)                            # the next call on any stream finds it cleared
         raise _lib.LrqkError(code, "lrqk_tree_attention", _lib.lib().lrqk_strerror(code).decode())
 
 

@@ -32,3 +32,19 @@ def test_the_cache_reports_it_where_it_reports_the_others():
             getattr(cache, how)()
         cache.check_status()                                       # looked at once
         cache.close()
+
+
+def test_a_look_waits_for_calls_on_other_streams():
+    word = _word()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)                             # some 50 ms of work ahead of the failing call
+        word.fill_(ETIMEOUT)
+    with pytest.raises(LrqkError):
+        check_tree_status()
+    q, ck, cv, tk, tv, _ = make(1, 2, 1, 1, 3, 9, 64, torch.bfloat16)
+    with torch.cuda.stream(side):                                  # and what it cleared is cleared for every stream
+        got = tree_attention(q, ck, cv, tk, tv, return_lse=True)
+    torch.cuda.synchronize()
+    check(got, q, ck, cv, tk, tv)
+    check_tree_status()
