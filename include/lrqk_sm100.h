@@ -403,8 +403,9 @@ int lrqk_rotary(const lrqk_rotary_args *a, lrqk_stream_t stream);
  *   mask       : bytes [nodes][nodes] per sequence, mask_stride bytes apart (0: one for all); NULL: node i sees 0..i.
  *   out        : dense [batch, q_heads, nodes, d]; lse: optional dense fp32 [batch, q_heads, nodes], natural
  *                logarithm of the sum of exponentials.  A row that sees nothing gives zeros and -infinity.
- *   status     : optional device int32, zero before the first call: takes LRQK_ETIMEOUT if a bounded wait ran out; as
- *                long as it is set, calls hand out NaN rows.
+ *   status     : device int32, zero before the first call: takes LRQK_ETIMEOUT if a bounded wait ran out; as
+ *                long as it is set, calls hand out NaN rows.  NULL: the call clears and uses a word of its workspace (one
+ *                more, small, operation on the stream), and its rows alone are NaN.
  *   head_dim 64 or 128, up to 256 nodes.  out and workspace start on 32 bytes; the workspace needs no initialisation.
  * ---------------------------------------------------------------------------------- */
 typedef struct lrqk_tree_args {

@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
   const int row = blockIdx.x * (8 / WARPS) + warp / WARPS;   // (batch * q_heads * nodes is below 2^31)
   const bool exists = row < p.batch * p.q_heads * p.nodes;
   const int t = row % p.nodes, h = row / p.nodes % p.q_heads, b = row / p.nodes / p.q_heads;
-  const int32_t broken = p.status ? *reinterpret_cast<volatile int32_t *>(p.status) : 0;
+  const int32_t broken = *reinterpret_cast<volatile int32_t *>(p.status);
   const Count n = count_tiles(p, b);
   T *dst = static_cast<T *>(p.out) + (int64_t)row * D + lane * E;
   const int per_head = p.q_heads / p.cache_heads, head = h / per_head;
@@ -354,7 +354,7 @@ int plan(const lrqk_tree_args *a, Params &p) {
 
 size_t workspace_bytes(const Params &p) {
   const size_t rows = (size_t)p.groups * 2 * p.row_blocks * p.rows_per_block;
-  return rows * p.head_dim * sizeof(float) + rows * sizeof(float2);
+  return rows * p.head_dim * sizeof(float) + rows * sizeof(float2) + sizeof(int32_t);   // partials; a status word
 }
 
 }  // namespace
@@ -404,6 +404,10 @@ int lrqk_tree_attention(const lrqk_tree_args *a, void *workspace, lrqk_stream_t 
   p.part = static_cast<float *>(workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part + (size_t)p.groups * 2 * p.row_blocks * p.rows_per_block * p.head_dim);
   const cudaStream_t s = as_stream(stream);
+  if (!p.status) {   // the call's own word: the combine kernel has to know of a wait that ran out, whoever else looks
+    p.status = reinterpret_cast<int32_t *>(static_cast<unsigned char *>(workspace) + tree::workspace_bytes(p) - sizeof(int32_t));
+    LRQK_CUDA_TRY(cudaMemsetAsync(p.status, 0, sizeof(int32_t), s));
+  }
   if (a->dtype == LRQK_BF16) rc = tree::launch_tc(p, s);
   else rc = a->head_dim == 64 ? tree::launch_simt<64>(p, s) : tree::launch_simt<128>(p, s);
   if (rc != LRQK_OK) return rc;

@@ -291,7 +291,7 @@ tree_tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params
   volatile uint32_t *give_up = &bar.give_up;
   const auto quit = [&]() {
     *give_up = 1;
-    if (p.status) atomicExch(p.status, (int32_t)LRQK_ETIMEOUT);
+    atomicExch(p.status, (int32_t)LRQK_ETIMEOUT);
   };
   const int per_head = p.q_heads / p.cache_heads, share = p.cache_heads / p.tree_heads;
   Walk w(p, bar.x0, bar.x1, bar.seq, bar.base);

@@ -23,7 +23,7 @@ struct Params {
   int64_t mask_stride;      // between sequences
   void *out;                // dense [batch][q_heads][nodes][head_dim]
   float *lse;               // dense [batch][q_heads][nodes] or null
-  int32_t *status;          // device word that takes LRQK_ETIMEOUT, or null
+  int32_t *status;          // device word that takes LRQK_ETIMEOUT
   float *part;              // partial rows: [slot][rows_per_block][head_dim], slot = (group * 2 + which) * row_blocks + block
   float2 *part_ml;          // [slot][rows_per_block]: maximum (base-2 logarithm units), sum
   float scale_log2;         // scale * log2(e)

@@ -42,7 +42,8 @@ _status: Dict[int, torch.Tensor] = {}
 
 def _status_word(device: torch.device) -> Optional[int]:
     """Address of the device's status word.  Made and cleared once, with a synchronisation so that every stream finds it
-    cleared; a first call under capture goes without one (its clearing would only run at the replays)."""
+    cleared; a first call under capture goes without one (its clearing would only run at the replays) and has one of its own,
+    cleared at every replay: its rows turn NaN all the same, but nobody is told."""
     word = _status.get(device.index)
     if word is None:
         if torch.cuda.is_current_stream_capturing():
@@ -56,7 +57,7 @@ def _status_word(device: torch.device) -> Optional[int]:
 def check_tree_status(device=None) -> None:
     """Synchronising look at the status word of a device's ``tree_attention`` calls, on whichever stream: raises
     ``LrqkError`` if a bounded wait of one ran out (its rows, and those of later calls until this look, are NaN), and
-    clears it."""
+    clears it.  A graph whose capture held the device's very first call has a word of its own that this look does not see."""
     index = torch.cuda.current_device() if device is None or torch.device(device).index is None else torch.device(device).index
     word = _status.get(index)
     if word is None:
