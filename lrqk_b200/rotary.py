@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .state import _DTYPES, call_on
+from .state import _DTYPES, call_on, has_tangent
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None, seq_len: Optional[int] = None,
@@ -107,12 +107,13 @@ def _rotate(q, k, positions, inv_freq, factor, interleaved, adjoint):
 
 
 class _Rotary(torch.autograd.Function):
-    """The rotation is linear: its gradient is the adjoint rotation of the gradients."""
+    """The rotation is linear: its gradient is the adjoint rotation of the gradients, its tangent that of the tangents."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, factor, interleaved, adjoint):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.how = (factor, interleaved, adjoint)
+        ctx.save_for_forward(positions, inv_freq)
+        ctx.how, ctx.two = (factor, interleaved, adjoint), k is not None
         q_out, k_out = _rotate(q, k, positions, inv_freq, factor, interleaved, adjoint)
         return (q_out,) if k is None else (q_out, k_out)
 
@@ -123,6 +124,13 @@ class _Rotary(torch.autograd.Function):
         got = apply_rotary(gq, gk, positions, inv_freq, factor=factor, interleaved=interleaved, adjoint=not adjoint)
         gq, gk = got if gk is not None else (got, None)
         return gq, gk, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, dq, dk, *_):
+        positions, inv_freq = ctx.saved_tensors
+        factor, interleaved, adjoint = ctx.how
+        turn = lambda x: None if x is None else apply_rotary(x, None, positions, inv_freq, factor=factor, interleaved=interleaved, adjoint=adjoint)  # noqa: E731
+        return (turn(dq), turn(dk)) if ctx.two else (turn(dq),)
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -135,7 +143,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     * ``adjoint``: turn backwards with the same factor, which is the gradient of the forward rotation
 
     Strided inputs (a transposed projection) are read as they are; the results are contiguous.  Differentiable in ``q`` and
-    ``k``.  Returns ``(q', k')``, or ``q'`` when ``k`` is ``None``."""
+    ``k``, backwards and in forward mode (dual tensors).  Returns ``(q', k')``, or ``q'`` when ``k`` is ``None``."""
     if q.dim() != 4 or q.dtype not in _DTYPES or not q.is_cuda:
         raise ValueError(f"q: expected a float32 or bfloat16 CUDA tensor [batch, heads, length, head_dim], got {q.dtype} {tuple(q.shape)} on {q.device}")
     b, _, n, d = q.shape
@@ -158,7 +166,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     factor = float(factor)
     if not math.isfinite(factor):
         raise ValueError(f"factor must be finite, got {factor}")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or has_tangent(q, k):
         got = _Rotary.apply(q, k, positions, inv_freq, factor, bool(interleaved), bool(adjoint))
         return got[0] if k is None else got
     got = _rotate(q, k, positions, inv_freq, factor, bool(interleaved), bool(adjoint))

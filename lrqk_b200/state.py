@@ -15,6 +15,7 @@ from typing import Optional, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -138,6 +139,14 @@ def call_on(device: torch.device, fn, *args) -> int:
         return fn(*args, _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream)
     with torch.cuda.device(index):
         return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def has_tangent(*tensors) -> bool:
+    """Is one of these (None among them) a dual tensor of forward-mode differentiation?  The kernels take addresses and would
+    drop the tangent.  (A look at the level first: unpacking takes half a microsecond each.)"""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return False
+    return any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)
 
 
 class LayerState:

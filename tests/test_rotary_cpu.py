@@ -77,3 +77,15 @@ def test_cpu_tensors_are_refused():
     x = torch.zeros(1, 2, 3, 64)
     with pytest.raises(ValueError):
         apply_rotary(x, None, torch.arange(3), inv)
+
+
+def test_dual_tensors_are_noticed():
+    from torch.autograd import forward_ad
+    from lrqk_b200.state import has_tangent
+    x = torch.ones(3)
+    assert not has_tangent(x, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        assert not dual.requires_grad and has_tangent(None, dual) and has_tangent(x, dual) and not has_tangent(x, None)
+        with torch.no_grad():
+            assert has_tangent(dual)
