@@ -13,7 +13,7 @@ from typing import Dict, Optional, Sequence, Union
 import torch
 
 from . import _lib
-from .state import _DTYPES, call_on
+from .state import _DTYPES, call_on, has_tangent
 
 MAX_NODES = 256
 
@@ -116,6 +116,8 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
         raise ValueError(f"head_dim must be 64 or 128, got {d}")
     if torch.is_grad_enabled() and (q.requires_grad or cache_k.requires_grad or cache_v.requires_grad or tree_k.requires_grad or tree_v.requires_grad):
         raise ValueError("tree_attention has no gradient: call it under torch.no_grad()")
+    if has_tangent(q, cache_k, cache_v, tree_k, tree_v):
+        raise ValueError("tree_attention has no forward-mode derivative: call it on the primals")
     scale = d ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite, got {scale}")

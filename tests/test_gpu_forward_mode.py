@@ -44,3 +44,16 @@ def test_function_transforms_are_refused_loudly():
     q, pos, inv = torch.ones(1, 1, 2, 8, device="cuda"), torch.arange(2, device="cuda"), rotary_frequencies(8, device="cuda")[0]
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: apply_rotary(x, None, pos, inv), (q,), (q,))
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_tree_attention_refuses_dual_tensors(which):
+    from lrqk_b200 import tree_attention
+    x = [torch.randn(1, 2, n, 64, device="cuda") for n in (3, 8, 8, 3, 3)]
+    want = tree_attention(*x)
+    with forward_ad.dual_level():
+        dual = list(x)
+        dual[which] = forward_ad.make_dual(x[which], torch.ones_like(x[which]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            tree_attention(*dual)
+        assert torch.equal(tree_attention(*x), want)               # a level alone changes nothing
