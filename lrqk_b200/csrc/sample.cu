@@ -7,7 +7,8 @@
 // Every one of these decisions is a comparison of sums, and a sum in fp32 decides differently from one in another order as
 // soon as a number falls near a border.  So weights are 45-bit whole numbers, W = round(2^44 w), from an exponential in
 // double (own: Taylor to the fourth order around 128 table values of 2^x, Tang's table method): whole-number sums have no
-// order, are the same for any cluster size, and agree with 64-bit floating sums to 2^-34 of the mass.
+// order, are the same for any cluster size, and agree with 64-bit floating sums to V 2^-45 of the largest weight for V tokens
+// (2^-28 for 128256: equal logits, whose roundings all go one way), to about sqrt(V) 2^-46 where roundings are independent (2^-37).
 //
 // A row's logits are read once, into the shared memory of the cluster's CTAs (1, 2, 4 or 8: enough SMs for few rows,
 // enough memory for large vocabularies).  Top-k and top-p look for the place in the descending order where a running count
