@@ -6,9 +6,11 @@
 // copied.  The adjoint (gradient) turns by -t.  All arithmetic is fp32, rounded once on the way out.
 //
 // Angles: a far position loses its angle in fp32 (t = 131072 rad is known to 2^-7 rad there).  Only t modulo a turn
-// matters, so a frequency is held in TURNS per position as a 64-bit binary fraction, F = round(2^64 w / 2 pi), and
+// matters, so a frequency is held in TURNS per position as a 64-bit binary fraction, F = 2^64 (w / 2 pi modulo 1), and
 // position * F modulo 2^64 -- one wrapping integer product, right for negative positions too -- is the angle's
-// fraction of a turn with an error of |position| 2^-65 turns.
+// fraction of a turn.  What is lost is lost in forming w / 2 pi in a double (a rounded constant, a rounded product): an
+// error of |position| ((w / 2 pi) 2^-52 + 2^-65) turns, 2^-37 of a turn at position 131072 for w = 1 and less for slower
+// pairs, where fp32 results resolve 2^-24.
 //
 // Bound: HBM.  q and k are read once and written once; the angles come from registers, not from cos/sin tables.  A
 // thread owns one 16-byte run of pairs of one token, computes its cosines and sines once and applies them to a run
