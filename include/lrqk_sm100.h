@@ -399,7 +399,8 @@ int lrqk_rotary(const lrqk_rotary_args *a, lrqk_stream_t stream);
  *   every row on 16 bytes.  tree_heads divides cache_heads divides q_heads: the resident rows of a decoding layer have cache_heads =
  *   q_heads, an ordinary cache cache_heads = tree_heads = the KV heads.
  *   cache_lens : device int32 [batch], read when the kernel runs and cut to [0, capacity]; NULL: capacity.  Rows behind
- *                a length are not used and may hold anything, as may nodes that no node sees.
+ *                a length are not used and may hold anything, as may nodes that no node sees.  An infinite value in a
+ *                filled row gives infinity or (bf16) NaN in that column.
  *   mask       : bytes [nodes][nodes] per sequence, mask_stride bytes apart (0: one for all); NULL: node i sees 0..i.
  *   out        : dense [batch, q_heads, nodes, d]; lse: optional dense fp32 [batch, q_heads, nodes], natural
  *                logarithm of the sum of exponentials.  A row that sees nothing gives zeros and -infinity.

@@ -23,8 +23,9 @@
 //
 // What bounds it, over two full contexts of 119157 rows and 8 cache heads (979 MB, 149.5 us at 6.55 TB/s), 4 query heads a
 // cache head: 164 us with 1 node, 169 with 8, 176 with 16 and 192 with 32: HBM, and with more rows the products and exponentials
-// beside it.  64 nodes, two row blocks: 318 us, 3000 cycles a tile and block.  The products need 1536 of them and the exponentials
-// 1024; the rest is the hand-over between a chain's products and its weights.
+// beside it.  64 nodes, two row blocks: 318 to 324 us, and 380 in continuous operation, where the power cap takes the clock
+// from 1965 to 1380 MHz: 65 % of the cycles with a product under way (1536 of 2400 a tile and block), 43 % of the exponential
+// unit's, the rest the hand-over between a chain's products and its weights.
 //
 // At 168 registers a thread (320 threads) the kernel spills 172 bytes and loads 260 again for head_dim 128, about 14 loads
 // from local memory a tile and warp.

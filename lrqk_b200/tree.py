@@ -86,7 +86,7 @@ def tree_attention(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor
     * ``mask``: bool (or uint8) [T, T] or [B, T, T], ``mask[i, j]``: node i sees node j (:func:`tree_mask`); ``None``: a
       chain, node i sees nodes 0..i
     * ``cache_lens``: int32 [B] on the device, read when the kernel runs (a captured call follows it), cut to [0, S];
-      ``None``: all S rows.  Rows behind a length may hold anything.
+      ``None``: all S rows.  Rows behind a length may hold anything (an infinite value before it gives infinity or NaN)
     * ``Ht`` divides ``Hc`` divides ``Hq``; query head h reads cache head ``h // (Hq / Hc)`` and drafted head
       ``h // (Hq / Ht)``
     * ``scale``: default ``d ** -0.5``; T up to 256, d 64 or 128, float32 or bfloat16

@@ -34,8 +34,9 @@ def test_accuracy_does_not_depend_on_the_rows_of_a_head(d, t, hq, hc):
         check_two_parts(out, lse, q, ck, cv, tk, tv, mask, lens)
 
 
-def test_more_row_blocks_than_multiprocessors():
-    """256 nodes of 80 query heads on one cache head: 20480 rows."""
-    q, ck, cv, tk, tv, mask = make(1, 80, 1, 1, 256, 200, 64, torch.bfloat16, seed=1, spread=0.5)
+@pytest.mark.parametrize("heads", [80, 256])
+def test_more_row_blocks_than_multiprocessors(heads):
+    """256 nodes of 80 and 256 query heads on one cache head: 20480 and 65536 rows, the most there are."""
+    q, ck, cv, tk, tv, mask = make(1, heads, 1, 1, 256, 200, 64, torch.bfloat16, seed=1, spread=0.5)
     out, lse = tree_attention(q, ck, cv, tk, tv, mask, return_lse=True)
     check_two_parts(out, lse, q, ck, cv, tk, tv, mask)
